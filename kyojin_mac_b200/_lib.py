@@ -160,6 +160,12 @@ SIGNATURES = {
     "kyb_gemv_group_t16": (_int, [_int, _vp, _vp, _i64, _i64, _int, _vp, _vp, _f32, _i64, _vp, _vp, _int, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp]),
     "kyb_gemv_plan": (_int, [_int, _i64, _i64, _i64, C.POINTER(C.c_int)]),
     "kyb_gemv_plan_within": (_int, [_int, _i64, _i64, _i64, _sz, C.POINTER(C.c_int)]),
+    "kyb_paged_step": (_int, [_vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _int, _i64] + [_vp] * 8),
+    "kyb_paged_release": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _i64, _vp, _vp, _vp]),
+    "kyb_rope_append": (_int, [_vp, _i64, _i64] * 3 + [_vp, _vp, _vp, _i64, _int, _int, _int, _int, _int, _f32, _int] + [_vp, _i64, _i64] * 3 + [_i64, _int, _vp]),
+    "kyb_paged_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _int, _int, _int, _int]),
+    "kyb_paged_attention": (_int, [_vp, _i64, _i64] * 3 + [_i64, _int, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _int, _int, _int, _int, _f32, _i64, _i64] + [_vp, _i64, _i64]
+                            + [_vp, _sz, _vp]),
     "kyb_check_device_status": (_int, [_vp]),
     "kyb_selftest_wait_timeout": (_int, [_int, _vp]),
 }

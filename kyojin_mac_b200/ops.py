@@ -1,6 +1,10 @@
 """Thin torch-tensor front end of the C ABI: pointers, sizes and the current CUDA stream go straight to libkyb.so."""
 from __future__ import annotations
 
+import contextlib
+import math
+from typing import NamedTuple
+
 import numpy as np
 import torch
 
@@ -487,3 +491,223 @@ def gemm_nvfp4(a_codes, sfa, b_codes, sfb, m: int, n: int, k: int, gscale: float
     _lib.check(_lib.lib().kyb_gemm_nvfp4(a_codes.data_ptr(), sfa.data_ptr(), b_codes.data_ptr(), sfb.data_ptr(), m, n, k, float(gscale), _DT[d.dtype], d.data_ptr(),
                                          d.stride(0), _stream()))
     return d
+
+
+# ------------------------------------------------------------------------------------------------ attention over a paged cache
+_NOGUARD = contextlib.nullcontext()
+
+
+def _place(*ts):
+    """The device guard of a call: all tensors on one CUDA device; that device current during the call."""
+    dev = ts[0].device
+    for t in ts:
+        if not t.is_cuda:
+            raise ValueError("kyojin_mac_b200 operators take CUDA tensors (there is no CPU path)")
+        if t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}: one device per call")
+    return _NOGUARD if _cur_device is not None and dev.index == _cur_device() else torch.cuda.device(dev)
+
+
+def _i32(t, name, *shape):
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != len(shape) or any(s is not None and s != n for s, n in zip(shape, t.shape)):
+        raise ValueError(f"{name} must be contiguous int32 [{', '.join('*' if s is None else str(s) for s in shape)}], got {t.dtype} {tuple(t.shape)}")
+
+
+def _table(t, page):
+    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] < 1 or t.shape[1] < 1 or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise ValueError(f"the block table is int32 [batch, columns] with dense rows, got {t.dtype} {tuple(t.shape)}")
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError("the block table's rows overlap")
+    if page not in (16, 32, 64, 128, 256):
+        raise ValueError(f"{page} tokens a page: 16, 32, 64, 128 or 256")
+
+
+def _heads(t, name):
+    """[tokens, heads, d] of a 16-bit type, heads dense, strides that 16-byte accesses can follow."""
+    if t.dtype not in (torch.float16, torch.bfloat16) or t.dim() != 3:
+        raise ValueError(f"{name} must be float16 or bfloat16 [tokens, heads, d], got {t.dtype} {tuple(t.shape)}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient: the paged cache serves inference (use torch.no_grad or detach)")
+    if t.numel() and (t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16):
+        raise ValueError(f"{name}: heads must be dense, strides multiples of 8 elements, the start 16-byte aligned; got strides {t.stride()}")
+
+
+def _cache(t, name, like=None):
+    if t.dtype not in (torch.float16, torch.bfloat16) or t.dim() != 4 or t.shape[2] not in (16, 32, 64, 128, 256) or (like is not None and (t.shape != like.shape or t.dtype != like.dtype)):
+        raise ValueError(f"{name} must be float16 or bfloat16 [pages, kv heads, 16 .. 256 (a power of two), d], keys and values alike, got {t.dtype} {tuple(t.shape)}")
+    p, h, n, d = t.shape
+    if t.numel() == 0 or t.stride(3) != 1 or t.stride(2) != d or t.data_ptr() % 16 or (p > 1 and (t.stride(0) % 8 or t.stride(0) < n * d)) or (h > 1 and (t.stride(1) % 8 or t.stride(1) < n * d)):
+        raise ValueError(f"{name}: the tokens of a page and head must be dense, strides multiples of 8 elements, the start 16-byte aligned; got strides {t.stride()}")
+
+
+class PagedStep(NamedTuple):
+    """What `paged_step` gives: int32 device tensors."""
+    cu_q: torch.Tensor          # [batch + 1] first row of each request
+    kv_lens: torch.Tensor       # [batch] tokens to attend over, the new ones included (0: not served)
+    positions: torch.Tensor     # [rows] place of each row's token in its request (-1: not served, or a row behind the last request)
+    slots: torch.Tensor         # [rows] place in the cache (-1 as above)
+    lens: torch.Tensor          # [batch] tokens held after the step
+    free_count: torch.Tensor    # [1] free pages left
+    refused: torch.Tensor       # [1] requests that could not be served
+
+
+def paged_step(table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor, page: int, rows: int,
+               in_place: bool = False) -> PagedStep:
+    """Slots of a step from request lengths, in one launch without a word to the host. Request r holds lens[r] tokens and brings new_lens[r] (packed in request order
+    into the step's `rows` rows); the pages it lacks come from the top of free_pages[:free_count] and are entered in its row of `table` [batch, columns].
+    A request is served when its pages fit the columns, its tokens the rows, and the needs of the requests up to its own the free list (one that needs no page
+    is not held up); `refused` counts the others, whose lengths stay. in_place: lens and free_count are updated too (a captured step that is replayed)."""
+    guard = _place(table, lens, new_lens, free_pages, free_count)
+    _table(table, page)
+    b, cols = table.shape
+    _i32(lens, "lens", b), _i32(new_lens, "new_lens", b), _i32(free_pages, "free_pages", None), _i32(free_count, "free_count", 1)
+    if free_pages.numel() < 1 or rows < 0:
+        raise ValueError("the free list is an array with room for a page at least, rows not negative")
+    with guard:
+        sizes = [b + 1, b, rows, rows, 1] + ([] if in_place else [b, 1])
+        cu, kv, pos, slots, refused, *more = lens.new_empty(sum(sizes)).split_with_sizes(sizes)
+        out_lens, out_count = (lens, free_count) if in_place else more
+        rc = _lib.lib().kyb_paged_step(lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), table.data_ptr(), max(table.stride(0), cols), b,
+                                       cols, page, rows, cu.data_ptr(), kv.data_ptr(), pos.data_ptr(), slots.data_ptr(), out_lens.data_ptr(), out_count.data_ptr(), refused.data_ptr(),
+                                       _stream())
+        if rc:
+            _lib.check(rc)
+    return PagedStep(cu, kv, pos, slots, out_lens, out_count, refused)
+
+
+def paged_release(table: torch.Tensor, lens: torch.Tensor, which: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor, page: int) -> torch.Tensor:
+    """The pages of the requests with which[r] (bool [batch]) go back to the free list, in place: their lengths become 0, their table entries -1. Returns int32 [1]:
+    requests whose pages would overflow the list (they keep them)."""
+    guard = _place(table, lens, which, free_pages, free_count)
+    _table(table, page)
+    b, cols = table.shape
+    _i32(lens, "lens", b), _i32(free_pages, "free_pages", None), _i32(free_count, "free_count", 1)
+    if which.dtype not in (torch.bool, torch.uint8) or which.shape != (b,) or not which.is_contiguous() or free_pages.numel() < 1:
+        raise ValueError(f"which must be bool [{b}], the free list an array with room for a page at least")
+    with guard:
+        refused = lens.new_empty(1)
+        _lib.check(_lib.lib().kyb_paged_release(lens.data_ptr(), which.data_ptr(), table.data_ptr(), max(table.stride(0), cols), b, cols, page, free_pages.data_ptr(), free_pages.numel(),
+                                                free_count.data_ptr(), refused.data_ptr(), _stream()))
+    return refused
+
+
+def rope_frequencies(rot: int, base: float = 10000.0, scaling: dict | None = None, device="cuda"):
+    """(inv_freq fp32 [rot / 2], mscale) of rotary positions: inv_freq[i] = base^(-2 i / rot), made in 64 bits. scaling, for contexts longer than the one trained on:
+    {"type": "linear", "factor"}: all frequencies divided by the factor;
+    {"type": "ntk", "factor"}: the base grown to base * factor^(rot / (rot - 2)), so that the slowest pair is divided by the factor and the fastest stays;
+    {"type": "llama3", "factor", "low_freq_factor", "high_freq_factor", "original_context"}: pairs of fewer than low_freq_factor turns in the original context divided by
+    the factor, of more than high_freq_factor kept, in between mixed linearly in the number of turns;
+    {"type": "yarn", "factor", "original_context", "beta_fast" (32), "beta_slow" (1)}: the same with a ramp over the pair's index, and mscale = 0.1 ln(factor) + 1."""
+    if rot < 16 or rot % 16:
+        raise ValueError(f"rot={rot}: a multiple of 16")
+    if not base > 1.0:
+        raise ValueError("the base is above 1")
+    i = torch.arange(0, rot, 2, dtype=torch.float64)
+    inv, mscale = base ** (-i / rot), 1.0
+    if scaling is not None:
+        kind, f = scaling.get("type"), float(scaling.get("factor", 0.0))
+        if not f >= 1.0 or not math.isfinite(f):
+            raise ValueError("a scaling has a factor of 1 at least")
+        if kind == "linear":
+            inv = inv / f
+        elif kind == "ntk":
+            inv = (base * f ** (rot / (rot - 2))) ** (-i / rot)
+        elif kind == "llama3":
+            low, high, ctx = (float(scaling[k]) for k in ("low_freq_factor", "high_freq_factor", "original_context"))
+            if not high > low:
+                raise ValueError("high_freq_factor is above low_freq_factor")
+            keep = ((ctx * inv / (2 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
+            inv = inv * keep + inv / f * (1 - keep)
+        elif kind == "yarn":
+            ctx, fast, slow = float(scaling["original_context"]), float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+            index = lambda turns: rot * math.log(ctx / (turns * 2 * math.pi)) / (2 * math.log(base))          # pair that makes so many turns in the context
+            a, b = max(math.floor(index(fast)), 0), min(math.ceil(index(slow)), rot - 1)
+            keep = 1.0 - ((torch.arange(rot // 2, dtype=torch.float64) - a) / max(b - a, 0.001)).clamp(0.0, 1.0)
+            inv, mscale = inv * keep + inv / f * (1 - keep), 0.1 * math.log(f) + 1.0
+        else:
+            raise ValueError(f"unknown scaling {kind!r}")
+    return inv.to(torch.float32).to(device), mscale
+
+
+def _rope_call(q, k, v, positions, slots, inv_freq, kc, vc, interleaved, mscale, out):
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq is contiguous float32 [rot / 2]")
+    T, hq, d = q.shape
+    if out is None:
+        out = q.new_empty((T, hq, d))
+    else:
+        _heads(out, "out")
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError("out has the queries' shape and type")
+    qs, os_, zero = q.stride(), out.stride(), (None, 0, 0)
+    kp, vp, kcp, vcp = zero, zero, zero, zero
+    hkv = pages = page = 0
+    if k is not None:
+        ks, vs, kcs, vcs = k.stride(), v.stride(), kc.stride(), vc.stride()
+        pages, hkv, page = kc.shape[:3]
+        kp, vp = (k.data_ptr(), ks[0], ks[1]), (v.data_ptr(), vs[0], vs[1])
+        kcp, vcp = (kc.data_ptr(), kcs[0], kcs[1]), (vc.data_ptr(), vcs[0], vcs[1])
+    rc = _lib.lib().kyb_rope_append(q.data_ptr(), qs[0], qs[1], *kp, *vp, positions.data_ptr(), None if slots is None else slots.data_ptr(), inv_freq.data_ptr(), T, hq, hkv, d,
+                                    2 * inv_freq.shape[0], 1 if interleaved else 0, mscale, _DT[q.dtype], out.data_ptr(), os_[0], os_[1], *kcp, *vcp, pages, page, _stream())
+    if rc:
+        _lib.check(rc)
+    return out
+
+
+def rope(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False, mscale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """x fp16 / bf16 [tokens, heads, d] with the first rot = 2 len(inv_freq) values of every head turned: pairs (i, i + rot / 2), or (2 i, 2 i + 1) when interleaved, by
+    positions[t] * inv_freq[i], scaled by mscale. Rows of a negative position are left as they are in `out` (which may be x)."""
+    guard = _place(x, positions, inv_freq, *(() if out is None else (out,)))
+    _heads(x, "x"), _i32(positions, "positions", x.shape[0])
+    with guard:
+        return _rope_call(x, None, None, positions, None, inv_freq, None, None, interleaved, float(mscale), out)
+
+
+def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, inv_freq: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                interleaved: bool = False, mscale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """`rope` of a step's queries, and in the same launch its keys (turned) and values into the cache [pages, kv heads, tokens of a page, d] at slots[t]. q [T, heads, d],
+    k and v [T, kv heads, d] may be views of one q | k | v product. Returns the turned queries. Rows with a negative position are left alone, a slot outside the cache
+    stores nothing; of rows that share a slot one is stored."""
+    guard = _place(q, k, v, positions, slots, inv_freq, k_cache, v_cache, *(() if out is None else (out,)))
+    _heads(q, "q"), _heads(k, "k"), _heads(v, "v"), _cache(k_cache, "k_cache"), _cache(v_cache, "v_cache", k_cache)
+    T, d = q.shape[0], q.shape[2]
+    if k.shape != (T, k_cache.shape[1], d) or v.shape != k.shape or k_cache.shape[3] != d or not q.dtype == k.dtype == v.dtype == k_cache.dtype:
+        raise ValueError(f"q [T, heads, d], k and v [T, kv heads, d] and the cache go together, in one type: got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}, {tuple(k_cache.shape)}")
+    _i32(positions, "positions", T), _i32(slots, "slots", T)
+    with guard:
+        return _rope_call(q, k, v, positions, slots, inv_freq, k_cache, v_cache, interleaved, float(mscale), out)
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, kv_lens: torch.Tensor, cu_q: torch.Tensor, max_q: int, scale: float | None = None,
+                    window: int = 0, sinks: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a step's new tokens over a paged cache: q fp16 / bf16 [T, heads, d] packed by request (rows [cu_q[r], cu_q[r + 1]); the last one is token
+    kv_lens[r] - 1), keys and values through the block table [batch, columns]. Causal; window > 0: the last `window` tokens only, and the first `sinks` ones.
+    max_q: the largest number of new tokens of a request (chooses the kernel; requests with more are served all the same). scale: d ** -0.5 unless given.
+    A row that sees nothing (kv_lens 0) gives zeros; rows behind the last request are left as they were (undefined without `out`). Returns out [T, heads, d]."""
+    guard = _place(q, k_cache, v_cache, table, kv_lens, cu_q, *(() if out is None else (out,)))
+    _heads(q, "q"), _cache(k_cache, "k_cache"), _cache(v_cache, "v_cache", k_cache)
+    (T, hq, d), (pages, hkv, page, dk) = q.shape, k_cache.shape
+    _table(table, page)
+    b, cols = table.shape
+    _i32(kv_lens, "kv_lens", b), _i32(cu_q, "cu_q", b + 1)
+    if d != dk or d not in (64, 128) or q.dtype != k_cache.dtype or hq % hkv or hq < hkv:
+        raise ValueError(f"heads of 64 or 128, a multiple of the cache's heads, in the cache's type: got q {q.dtype} {tuple(q.shape)}, cache {k_cache.dtype} {tuple(k_cache.shape)}")
+    if max_q < 0 or window < 0 or sinks < 0 or (sinks and not window):
+        raise ValueError("max_q, window and sinks are not negative, sinks come with a window")
+    with guard:
+        if out is None:
+            out = q.new_empty((T, hq, d))
+        else:
+            _heads(out, "out")
+            if out.shape != q.shape or out.dtype != q.dtype:
+                raise ValueError("out has the queries' shape and type")
+        L = _lib.lib()
+        need = L.kyb_paged_attention_workspace_bytes(b, T, max_q, cols, page, hq, hkv, d)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None    # the call's own: captured graphs that replay side by side share nothing
+        qs, os_, ks, vs = q.stride(), out.stride(), k_cache.stride(), v_cache.stride()
+        rc = L.kyb_paged_attention(q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), ks[0], ks[1], v_cache.data_ptr(), vs[0], vs[1], pages, page, table.data_ptr(),
+                                   max(table.stride(0), cols), cols, kv_lens.data_ptr(), cu_q.data_ptr(), b, T, max_q, hq, hkv, d, _DT[q.dtype], d ** -0.5 if scale is None else scale,
+                                   window, sinks, out.data_ptr(), os_[0], os_[1], None if ws is None else ws.data_ptr(), need, _stream())
+        if rc:
+            _lib.check(rc)
+    return out
