@@ -60,6 +60,7 @@ __host__ __device__ constexpr bool kyb_has_mins16(int fmt) { return fmt == KYB_F
 // status codes written to the device status word by kernels whose bounded wait expired
 #define KYB_DEV_TIMEOUT_GEMV 0x1001u
 #define KYB_DEV_TIMEOUT_GEMM 0x1002u
+#define KYB_DEV_TIMEOUT_ATTN 0x1003u
 #define KYB_DEV_TIMEOUT_SELFTEST 0x10FFu
 
 #ifdef __CUDACC__

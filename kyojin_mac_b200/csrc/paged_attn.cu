@@ -2,23 +2,14 @@
 // and with a window W only when j > p - W or j < sinks. Tokens of all requests are packed (cu_q), a request's last token is its last cached one.
 #include <algorithm>
 
-#include <cuda_bf16.h>
-
-#include "kyb_common.cuh"
+#include "paged_attn.cuh"
 
 namespace kyb {
 
-struct AttnParams {
-    const uint8_t *q, *k, *v;                                 // 16-bit elements
-    uint8_t* o;
-    int64_t q_t, q_h, o_t, o_h, k_p, k_h, v_p, v_h;           // strides in elements (token, head; page, head)
-    const int* table;
-    int64_t ld_table, cols, pages;
-    const int* kv_lens;
-    const int* cu_q;
-    int batch, page_log2, hq, hkv;
-    int64_t tokens, window, sinks;
-    float scale;
+struct SimpleParams {
+    AttnParams a;
+    const uint8_t *k, *v;
+    int64_t k_p, k_h, v_p, v_h;
 };
 
 template <typename T> __device__ __forceinline__ float as_float(T v);
@@ -30,7 +21,8 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { retur
 
 // One CTA per (token, query head); its four warps take every fourth key, each with its own running maximum and sum.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) paged_attn_simple_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(128) paged_attn_simple_kernel(const SimpleParams c) {
+    const AttnParams& p = c.a;
     constexpr int E = D / 32;
     __shared__ float so[4][D], sm[4], sl[4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -42,11 +34,11 @@ __global__ void __launch_bounds__(128) paged_attn_simple_kernel(const AttnParams
         if (p.cu_q[mid] <= t) lo = mid; else hi = mid;
     }
     if (t < p.cu_q[0] || t >= p.cu_q[lo + 1]) return;
-    const int64_t kv = min((int64_t)p.kv_lens[lo], p.cols << p.page_log2), pos = (int64_t)p.kv_lens[lo] - (p.cu_q[lo + 1] - t);
-    const int64_t end = min(pos + 1, kv), start = p.window ? max((int64_t)0, pos - p.window + 1) : 0, sink_end = min(p.sinks, start);
+    const int64_t pos = (int64_t)request_keys(p, lo) - (p.cu_q[lo + 1] - t);
+    const int64_t end = min(pos + 1, (int64_t)p.cap), start = p.window ? max((int64_t)0, pos - p.window + 1) : 0, sink_end = min((int64_t)p.sinks, start);
     const T* q = (const T*)p.q + t * p.q_t + h * p.q_h;
     float qr[E], o[E] = {};
-    for (int e = 0; e < E; ++e) qr[e] = as_float(q[lane * E + e]) * p.scale;
+    for (int e = 0; e < E; ++e) qr[e] = as_float(q[lane * E + e]) * p.scale2;
     float m = -INFINITY, l = 0.f;
     const int64_t n = sink_end + max((int64_t)0, end - start);
     for (int64_t i = warp; i < n; i += 4) {
@@ -54,12 +46,12 @@ __global__ void __launch_bounds__(128) paged_attn_simple_kernel(const AttnParams
         if (j >= end) continue;
         const int64_t id = p.table[lo * p.ld_table + (j >> p.page_log2)], off = (j & ((1 << p.page_log2) - 1)) * D + lane * E;
         const bool held = id >= 0 && id < p.pages;            // an entry that is no page reads as zeros
-        const T* kr = (const T*)p.k + (held ? id : 0) * p.k_p + hk * p.k_h + off;
-        const T* vr = (const T*)p.v + (held ? id : 0) * p.v_p + hk * p.v_h + off;
+        const T* kr = (const T*)c.k + (held ? id : 0) * c.k_p + hk * c.k_h + off;
+        const T* vr = (const T*)c.v + (held ? id : 0) * c.v_p + hk * c.v_h + off;
         float s = 0.f;
         for (int e = 0; e < E; ++e) s += qr[e] * (held ? as_float(kr[e]) : 0.f);
         for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        const float top = fmaxf(m, s), c = m == top ? 1.f : expf(m - top), w = expf(s - top);
+        const float top = fmaxf(m, s), c = m == top ? 1.f : exp2f(m - top), w = exp2f(s - top);
         l = l * c + w, m = top;
         for (int e = 0; e < E; ++e) o[e] = o[e] * c + w * (held ? as_float(vr[e]) : 0.f);
     }
@@ -70,7 +62,7 @@ __global__ void __launch_bounds__(128) paged_attn_simple_kernel(const AttnParams
     for (int x = threadIdx.x; x < D; x += 128) {
         float a = 0.f, b = 0.f;
         for (int w = 0; w < 4; ++w) {
-            const float c = sl[w] > 0.f ? expf(sm[w] - top) : 0.f;
+            const float c = sl[w] > 0.f ? exp2f(sm[w] - top) : 0.f;
             a += c * so[w][x], b += c * sl[w];
         }
         ((T*)p.o)[t * p.o_t + h * p.o_h + x] = from_float<T>(b > 0.f ? a / b : 0.f);
@@ -79,23 +71,31 @@ __global__ void __launch_bounds__(128) paged_attn_simple_kernel(const AttnParams
 
 }  // namespace kyb
 
+static int sm_count() {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    return n;
+}
+
 extern "C" size_t kyb_paged_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t max_q, int64_t cols, int page, int hq, int hkv, int d) {
-    (void)batch, (void)tokens, (void)max_q, (void)cols, (void)page, (void)hq, (void)hkv, (void)d;
-    return 0;
+    (void)batch, (void)cols, (void)page;
+    if (tokens <= 0 || hkv <= 0 || hq < hkv) return 0;
+    const int64_t rows = std::max<int64_t>(max_q, 1) * (hq / hkv);
+    return rows <= KYB_DECODE_ROWS ? kyb_attn_decode_scratch(d, (int)rows, sm_count()) : 0;
 }
 
 extern "C" int kyb_paged_attention(const void* q, int64_t q_t, int64_t q_h, const void* k_cache, int64_t k_page, int64_t k_head, const void* v_cache, int64_t v_page, int64_t v_head,
                                    int64_t pages, int page, const void* table, int64_t ld_table, int64_t cols, const void* kv_lens, const void* cu_q, int64_t batch, int64_t tokens,
                                    int64_t max_q, int hq, int hkv, int d, int dtype, float scale, int64_t window, int64_t sinks, void* out, int64_t o_t, int64_t o_h, void* ws,
                                    size_t ws_bytes, void* stream) {
-    KYB_REQUIRE(batch > 0 && batch < (1ll << 24) && tokens >= 0 && tokens < (1ll << 31) && max_q >= 0, "batch=%lld tokens=%lld max_q=%lld: out of range", (long long)batch, (long long)tokens,
+    KYB_REQUIRE(batch > 0 && batch < (1ll << 24) && tokens >= 0 && tokens < (1ll << 30) && max_q >= 0, "batch=%lld tokens=%lld max_q=%lld: out of range", (long long)batch, (long long)tokens,
                 (long long)max_q);
     KYB_REQUIRE(hkv > 0 && hq > 0 && hq % hkv == 0 && hq / hkv <= 128 && hkv <= 65535 && hq <= 65535, "heads %d / %d: query heads are a multiple (up to 128) of the key-value heads", hq, hkv);
     KYB_REQUIRE(d == 64 || d == 128, "d=%d: heads of 64 or 128", d);
     KYB_REQUIRE(dtype == 1 || dtype == 2, "dtype=%d: 1 (fp16) or 2 (bf16)", dtype);
-    KYB_REQUIRE(page >= 16 && page <= 256 && (page & (page - 1)) == 0 && pages > 0 && pages < (1ll << 31), "page=%d pages=%lld: a power of two from 16 to 256, at least one page", page,
+    KYB_REQUIRE(page >= 16 && page <= 256 && (page & (page - 1)) == 0 && pages > 0 && pages < (1ll << 31) - 1, "page=%d pages=%lld: a power of two from 16 to 256, at least one page", page,
                 (long long)pages);
-    KYB_REQUIRE(cols > 0 && ld_table >= cols && cols * page < (1ll << 31), "table of %lld columns (row stride %lld), %d tokens a page: out of range", (long long)cols, (long long)ld_table, page);
+    KYB_REQUIRE(cols > 0 && ld_table >= cols && cols <= (1 << 30) / page, "table of %lld columns (row stride %lld), %d tokens a page: out of range", (long long)cols, (long long)ld_table, page);
     KYB_REQUIRE(window >= 0 && sinks >= 0 && (window > 0 || sinks == 0), "window=%lld sinks=%lld: not negative, sinks only with a window", (long long)window, (long long)sinks);
     KYB_REQUIRE(scale == scale && scale - scale == 0.f, "the scale is a finite number");
     if (tokens == 0) return KYB_OK;
@@ -103,22 +103,37 @@ extern "C" int kyb_paged_attention(const void* q, int64_t q_t, int64_t q_h, cons
     const int64_t strides[] = {q_t, q_h, k_page, k_head, v_page, v_head, o_t, o_h};
     for (int64_t s : strides) KYB_REQUIRE(s % 8 == 0 && s >= 0, "a stride of %lld elements: strides are multiples of 8 elements (16 bytes)", (long long)s);
     KYB_REQUIRE((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15) == 0, "pointers must be 16-byte aligned");
-    kyb::AttnParams p;
-    p.q = (const uint8_t*)q, p.k = (const uint8_t*)k_cache, p.v = (const uint8_t*)v_cache, p.o = (uint8_t*)out;
-    p.q_t = q_t, p.q_h = q_h, p.o_t = o_t, p.o_h = o_h, p.k_p = k_page, p.k_h = k_head, p.v_p = v_page, p.v_h = v_head;
-    p.table = (const int*)table, p.ld_table = ld_table, p.cols = cols, p.pages = pages, p.kv_lens = (const int*)kv_lens, p.cu_q = (const int*)cu_q;
-    p.batch = (int)batch, p.hq = hq, p.hkv = hkv, p.tokens = tokens, p.window = window, p.sinks = sinks, p.scale = scale;
-    p.page_log2 = 0;
+    unsigned int* status = kyb_device_status_word();
+    KYB_REQUIRE(status, "could not set up the device status word");
+    KybAttnCall c;
+    kyb::AttnParams& p = c.p;
+    p.q = (const uint8_t*)q, p.o = (uint8_t*)out, p.q_t = q_t, p.q_h = q_h, p.o_t = o_t, p.o_h = o_h;
+    p.table = (const int*)table, p.ld_table = ld_table, p.kv_lens = (const int*)kv_lens, p.cu_q = (const int*)cu_q;
+    p.batch = (int)batch, p.tokens = (int)tokens, p.hq = hq, p.hkv = hkv, p.group = hq / hkv, p.pages = (int)pages, p.cap = (int)(cols * page);
+    p.window = (int)std::min<int64_t>(window, 1 << 30), p.sinks = (int)std::min<int64_t>(sinks, 1 << 30), p.scale2 = scale * 1.4426950408889634f, p.status = status;
+    p.page_log2 = 0, p.parts = nullptr, p.notes = nullptr;
     while ((1 << p.page_log2) < page) ++p.page_log2;
-    (void)ws, (void)ws_bytes;
+    c.k = k_cache, c.v = v_cache, c.k_p = k_page, c.k_h = k_head, c.v_p = v_page, c.v_h = v_head, c.tokens = tokens, c.d = d, c.dtype = dtype, c.page = page, c.sms = sm_count();
+    c.st = (cudaStream_t)stream;
+    KYB_REQUIRE(c.sms > 0, "no CUDA device");
+    const size_t need = kyb_paged_attention_workspace_bytes(batch, tokens, max_q, cols, page, hq, hkv, d);
+    if (ws_bytes < need || (need && !ws)) {
+        kyb_set_error("workspace of %zu bytes, %zu needed", ws_bytes, need);
+        return KYB_EWORKSPACE;
+    }
+    KYB_REQUIRE(!need || ((uintptr_t)ws & 15) == 0, "the workspace must be 16-byte aligned");
+    const int64_t rows = std::max<int64_t>(max_q, 1) * p.group;
+    if (rows <= KYB_DECODE_ROWS) return kyb_attn_decode(c, (int)rows, ws);
+    kyb::SimpleParams sp;
+    sp.a = p, sp.k = (const uint8_t*)k_cache, sp.v = (const uint8_t*)v_cache, sp.k_p = k_page, sp.k_h = k_head, sp.v_p = v_page, sp.v_h = v_head;
     const dim3 grid((unsigned)tokens, (unsigned)hq);
     cudaStream_t st = (cudaStream_t)stream;
     if (dtype == 1) {
-        if (d == 64) kyb::paged_attn_simple_kernel<__half, 64><<<grid, 128, 0, st>>>(p);
-        else kyb::paged_attn_simple_kernel<__half, 128><<<grid, 128, 0, st>>>(p);
+        if (d == 64) kyb::paged_attn_simple_kernel<__half, 64><<<grid, 128, 0, st>>>(sp);
+        else kyb::paged_attn_simple_kernel<__half, 128><<<grid, 128, 0, st>>>(sp);
     } else {
-        if (d == 64) kyb::paged_attn_simple_kernel<__nv_bfloat16, 64><<<grid, 128, 0, st>>>(p);
-        else kyb::paged_attn_simple_kernel<__nv_bfloat16, 128><<<grid, 128, 0, st>>>(p);
+        if (d == 64) kyb::paged_attn_simple_kernel<__nv_bfloat16, 64><<<grid, 128, 0, st>>>(sp);
+        else kyb::paged_attn_simple_kernel<__nv_bfloat16, 128><<<grid, 128, 0, st>>>(sp);
     }
     return kyb_launch_check("paged_attention");
 }

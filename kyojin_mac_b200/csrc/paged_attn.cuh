@@ -1,0 +1,166 @@
+// Attention over a paged cache: what the decode and the prefill kernel share (parameters, the keys that a block of rows sees, tensor maps of the cache, the split of the
+// work over the CTAs and the sum of the parts).
+//
+// Rows: the (token, query head) pairs of one request and one key-value head, token by token, G = hq / hkv rows a token: all of them read the same keys. A row block
+// is `block` consecutive ones. An item is (request, row block, key-value head); its work is cut along the keys into tiles of `tile` keys. The tiles of all items, in
+// order (request, then row block, then head), are dealt to the CTAs in equal contiguous runs, so ragged lengths and few long ones balance alike; an item that a run's
+// border cuts leaves parts in the scratch, unnormalised and in 32 bits, which a second launch adds in their order. Nothing depends on timing.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "tc_common.cuh"
+
+namespace kyb {
+
+struct AttnParams {
+    const uint8_t* q;                                         // 16-bit elements
+    uint8_t* o;
+    int64_t q_t, q_h, o_t, o_h;                               // strides in elements (token, head)
+    const int* table;
+    const int* kv_lens;
+    const int* cu_q;
+    int64_t ld_table;
+    int batch, tokens, hq, hkv, group, page_log2, pages, cap; // tokens: rows of q; cap: tokens that a row of the table can hold
+    int window, sinks;                                        // window 0: none
+    float scale2;                                             // scale log2(e)
+    unsigned int* status;
+    float* parts;                                             // scratch: parts[cta][2][block * (d + 2)]
+    int4* notes;                                              // scratch: notes[cta] = {request, row block, head, flags}
+};
+// flags of a CTA's note: its first run continues an item (and ends it), its last run begins an item that the next CTA continues
+constexpr int NOTE_CONTINUES = 1, NOTE_ENDS = 2, NOTE_BEGINS = 4;
+
+#ifdef __CUDACC__
+// The keys that a block of rows sees: tiles of `tile` keys, first those of the sinks, then those of the window (or of the whole context).
+struct KeySpan {
+    int row0, rows;            // first row of the block in its request, rows of the block
+    int first, last;           // positions of its first and last token
+    int lo, end;               // keys [lo, end) and [0, min(sinks, lo)) are seen by some row
+    int sink_tiles, main_tile, n;
+    __device__ __forceinline__ int tile(int i) const { return i < sink_tiles ? i : main_tile + (i - sink_tiles); }
+    __device__ __forceinline__ bool alive(int key, int sinks) const { return key < end && (key >= lo || key < sinks); }
+};
+
+__device__ __forceinline__ KeySpan key_span(const AttnParams& p, int tokens, int kv, int block, int rb, int tile) {
+    KeySpan s;
+    s.row0 = rb * block, s.rows = min(block, tokens * p.group - s.row0);
+    s.first = kv - tokens + s.row0 / p.group, s.last = kv - tokens + (s.row0 + s.rows - 1) / p.group;
+    s.end = max(0, min(s.last + 1, p.cap));
+    s.lo = p.window ? max(0, s.first - p.window + 1) : 0;
+    s.main_tile = s.lo / tile;
+    const int main_end = (s.end + tile - 1) / tile;
+    s.sink_tiles = min((min(p.sinks, s.end) + tile - 1) / tile, min(s.main_tile, main_end));
+    s.n = max(1, s.sink_tiles + max(0, main_end - s.main_tile));            // a block that sees nothing still has its zeros to write: one tile, masked throughout
+    return s;
+}
+// a request's first row and its rows, whatever cu_q holds: inside [0, tokens)
+__device__ __forceinline__ int request_rows(const AttnParams& p, int r, int& base) {
+    base = min(max(p.cu_q[r], 0), p.tokens);
+    return min(max(p.cu_q[r + 1], base), p.tokens) - base;
+}
+__device__ __forceinline__ int request_keys(const AttnParams& p, int r) { return min(max(p.kv_lens[r], 0), 1 << 30); }
+__device__ __forceinline__ int row_blocks(const AttnParams& p, int tokens, int block) { return (int)(((long long)max(0, tokens) * p.group + block - 1) / block); }
+
+// Tiles of one key-value head of a request
+__device__ __forceinline__ long long request_tiles(const AttnParams& p, int r, int block, int tile, int lane = 0, int lanes = 1) {
+    int base;
+    const int tokens = request_rows(p, r, base), kv = request_keys(p, r), nb = row_blocks(p, tokens, block);
+    long long n = 0;
+    for (int b = lane; b < nb; b += lanes) n += key_span(p, tokens, kv, block, b, tile).n;
+    return n;
+}
+
+// Where a CTA's run of tiles is: the item it starts in, and how many tiles it has
+struct Cursor {
+    int r, rb, h, at;          // request, row block, head, next tile of the item
+    long long left;            // tiles left in the run
+    int tokens, kv, blocks, row_base;
+    KeySpan s;
+    __device__ __forceinline__ void load(const AttnParams& p, int block, int tile) {
+        tokens = request_rows(p, r, row_base), kv = request_keys(p, r), blocks = row_blocks(p, tokens, block);
+        if (rb < blocks) s = key_span(p, tokens, kv, block, rb, tile);
+    }
+    // behind an item: to the next one
+    __device__ __forceinline__ void next(const AttnParams& p, int block, int tile) {
+        at = 0;
+        if (++h < p.hkv) return;
+        h = 0, ++rb;
+        while (rb >= blocks) {
+            rb = 0;
+            if (++r >= p.batch) {
+                left = 0;
+                return;
+            }
+            load(p, block, tile);
+        }
+        s = key_span(p, tokens, kv, block, rb, tile);
+    }
+};
+
+// 5-D copy of a piece of one page and head into shared memory: [half of the values][token][128 bytes], 128-byte swizzle
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* tm, int x, int y, int z, int h, int page, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst), "l"(tm), "r"(x), "r"(y), "r"(z), "r"(h),
+                 "r"(page), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a));
+    return d;
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    uint32_t d;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a));
+    return d;
+}
+#endif
+
+}  // namespace kyb
+
+// tensor map of a cache [pages][heads][page][d] of 16-bit values: {64 values, token, half, head, page}, boxes of `box_tokens` tokens and `box_halves` halves
+static inline int kyb_make_cache_map(CUtensorMap* tm, const void* base, int dtype, int64_t pages, int heads, int page, int d, int64_t page_stride, int64_t head_stride, int box_tokens,
+                                     int box_halves) {
+    kyb_encode_tiled_fn enc = kyb_get_encode_tiled();
+    if (!enc) {
+        kyb_set_error("cuTensorMapEncodeTiled is not available from this driver");
+        return KYB_ECUDA;
+    }
+    if (heads == 1) head_stride = (int64_t)page * d;                        // the stride of a dimension of one is never used: any valid one
+    if (pages == 1) page_stride = head_stride * heads;
+    const cuuint64_t dims[5] = {64, (cuuint64_t)page, (cuuint64_t)(d / 64), (cuuint64_t)heads, (cuuint64_t)pages};
+    const cuuint64_t strides[4] = {(cuuint64_t)d * 2, 128, (cuuint64_t)head_stride * 2, (cuuint64_t)page_stride * 2};
+    const cuuint32_t box[5] = {64, (cuuint32_t)box_tokens, (cuuint32_t)box_halves, 1, 1}, estr[5] = {1, 1, 1, 1, 1};
+    const CUresult r = enc(tm, dtype == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(base), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        kyb_set_error("cuTensorMapEncodeTiled failed with CUresult %d (cache %p: %lld pages, %d heads, %d tokens of %d values, strides %lld, %lld)", (int)r, base, (long long)pages, heads, page,
+                      d, (long long)page_stride, (long long)head_stride);
+        return KYB_ECUDA;
+    }
+    return KYB_OK;
+}
+
+// The call as the C entry hands it to a kernel's launcher
+struct KybAttnCall {
+    kyb::AttnParams p;
+    const void *k, *v;
+    int64_t k_p, k_h, v_p, v_h, tokens;
+    int d, dtype, page, sms;
+    cudaStream_t st;
+};
+// rows a request may bring for the decode kernel; beyond, the prefill kernel
+constexpr int KYB_DECODE_ROWS = 16;
+size_t kyb_attn_decode_scratch(int d, int rows, int sms);
+int kyb_attn_decode(KybAttnCall& c, int rows, void* ws);
+// second launch: adds the parts of the items that were cut (ctas runs, blocks of `block` rows)
+int kyb_attn_join(const KybAttnCall& c, int ctas, int block);

@@ -52,7 +52,7 @@ def test_attention_refusals(lib):
                 dt=1, scale=0.1, window=0, sinks=0, out=P, o_t=128, o_h=64, ws=P, wsn=1 << 30)
     call = lambda **k: lib.kyb_paged_attention(*{**good, **k}.values(), None)
     for bad in (dict(q=None), dict(v=None), dict(table=None), dict(out=None), dict(q=P + 2), dict(out=P + 4), dict(q_t=100), dict(k_p=1028), dict(o_h=-64), dict(pages=0), dict(pages=1 << 31),
-                dict(page=8), dict(page=100), dict(ld=2), dict(cols=0), dict(cols=1 << 28, ld=1 << 28), dict(batch=0), dict(tokens=-1), dict(tokens=1 << 31), dict(max_q=-1), dict(hq=0),
+                dict(page=8), dict(page=100), dict(ld=2), dict(cols=0), dict(cols=1 << 28, ld=1 << 28), dict(batch=0), dict(tokens=-1), dict(tokens=1 << 30), dict(max_q=-1), dict(hq=0),
                 dict(hq=3, hkv=2), dict(hq=129), dict(d=96), dict(dt=0), dict(scale=math.nan), dict(scale=math.inf), dict(window=-1), dict(sinks=-1), dict(sinks=4)):
         assert call(**bad) == _lib.EINVAL, bad
     assert call(tokens=0) == _lib.OK
