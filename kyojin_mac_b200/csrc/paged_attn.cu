@@ -1,75 +1,10 @@
 // Attention of a step's new tokens over a paged cache: o = softmax(scale q K^T) V per query head, where the token at position p of its request sees key j when j <= p,
 // and with a window W only when j > p - W or j < sinks. Tokens of all requests are packed (cu_q), a request's last token is its last cached one.
+#include <float.h>
+
 #include <algorithm>
 
 #include "paged_attn.cuh"
-
-namespace kyb {
-
-struct SimpleParams {
-    AttnParams a;
-    const uint8_t *k, *v;
-    int64_t k_p, k_h, v_p, v_h;
-};
-
-template <typename T> __device__ __forceinline__ float as_float(T v);
-template <> __device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
-
-// One CTA per (token, query head); its four warps take every fourth key, each with its own running maximum and sum.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) paged_attn_simple_kernel(const SimpleParams c) {
-    const AttnParams& p = c.a;
-    constexpr int E = D / 32;
-    __shared__ float so[4][D], sm[4], sl[4];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t t = blockIdx.x;
-    const int h = blockIdx.y, hk = h / (p.hq / p.hkv);
-    int lo = 0, hi = p.batch;                                 // request: the last r with cu_q[r] <= t (requests without tokens repeat a value)
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (p.cu_q[mid] <= t) lo = mid; else hi = mid;
-    }
-    if (t < p.cu_q[0] || t >= p.cu_q[lo + 1]) return;
-    const int64_t pos = (int64_t)request_keys(p, lo) - (p.cu_q[lo + 1] - t);
-    const int64_t end = min(pos + 1, (int64_t)p.cap), start = p.window ? max((int64_t)0, pos - p.window + 1) : 0, sink_end = min((int64_t)p.sinks, start);
-    const T* q = (const T*)p.q + t * p.q_t + h * p.q_h;
-    float qr[E], o[E] = {};
-    for (int e = 0; e < E; ++e) qr[e] = as_float(q[lane * E + e]) * p.scale2;
-    float m = -INFINITY, l = 0.f;
-    const int64_t n = sink_end + max((int64_t)0, end - start);
-    for (int64_t i = warp; i < n; i += 4) {
-        const int64_t j = i < sink_end ? i : start + (i - sink_end);
-        if (j >= end) continue;
-        const int64_t id = p.table[lo * p.ld_table + (j >> p.page_log2)], off = (j & ((1 << p.page_log2) - 1)) * D + lane * E;
-        const bool held = id >= 0 && id < p.pages;            // an entry that is no page reads as zeros
-        const T* kr = (const T*)c.k + (held ? id : 0) * c.k_p + hk * c.k_h + off;
-        const T* vr = (const T*)c.v + (held ? id : 0) * c.v_p + hk * c.v_h + off;
-        float s = 0.f;
-        for (int e = 0; e < E; ++e) s += qr[e] * (held ? as_float(kr[e]) : 0.f);
-        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        const float top = fmaxf(m, s), c = m == top ? 1.f : exp2f(m - top), w = exp2f(s - top);
-        l = l * c + w, m = top;
-        for (int e = 0; e < E; ++e) o[e] = o[e] * c + w * (held ? as_float(vr[e]) : 0.f);
-    }
-    for (int e = 0; e < E; ++e) so[warp][lane * E + e] = o[e];
-    if (lane == 0) sm[warp] = m, sl[warp] = l;
-    __syncthreads();
-    const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-    for (int x = threadIdx.x; x < D; x += 128) {
-        float a = 0.f, b = 0.f;
-        for (int w = 0; w < 4; ++w) {
-            const float c = sl[w] > 0.f ? exp2f(sm[w] - top) : 0.f;
-            a += c * so[w][x], b += c * sl[w];
-        }
-        ((T*)p.o)[t * p.o_t + h * p.o_h + x] = from_float<T>(b > 0.f ? a / b : 0.f);
-    }
-}
-
-}  // namespace kyb
 
 static int sm_count() {
     int dev = 0, n = 0;
@@ -79,9 +14,9 @@ static int sm_count() {
 
 extern "C" size_t kyb_paged_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t max_q, int64_t cols, int page, int hq, int hkv, int d) {
     (void)batch, (void)cols, (void)page;
-    if (tokens <= 0 || hkv <= 0 || hq < hkv) return 0;
+    if (tokens <= 0 || hkv <= 0 || hq < hkv || hq / hkv > 128) return 0;
     const int64_t rows = std::max<int64_t>(max_q, 1) * (hq / hkv);
-    return rows <= KYB_DECODE_ROWS ? kyb_attn_decode_scratch(d, (int)rows, sm_count()) : 0;
+    return rows <= KYB_DECODE_ROWS ? kyb_attn_decode_scratch(d, (int)rows, sm_count()) : kyb_attn_prefill_scratch(d, hq / hkv, sm_count());
 }
 
 extern "C" int kyb_paged_attention(const void* q, int64_t q_t, int64_t q_h, const void* k_cache, int64_t k_page, int64_t k_head, const void* v_cache, int64_t v_page, int64_t v_head,
@@ -111,6 +46,8 @@ extern "C" int kyb_paged_attention(const void* q, int64_t q_t, int64_t q_h, cons
     p.table = (const int*)table, p.ld_table = ld_table, p.kv_lens = (const int*)kv_lens, p.cu_q = (const int*)cu_q;
     p.batch = (int)batch, p.tokens = (int)tokens, p.hq = hq, p.hkv = hkv, p.group = hq / hkv, p.pages = (int)pages, p.cap = (int)(cols * page);
     p.window = (int)std::min<int64_t>(window, 1 << 30), p.sinks = (int)std::min<int64_t>(sinks, 1 << 30), p.scale2 = scale * 1.4426950408889634f, p.status = status;
+    // a hidden score is -inf and stays so times the scale: 0 would make it NaN, the smallest normal number gives the same weights
+    if (!(p.scale2 >= FLT_MIN || p.scale2 <= -FLT_MIN)) p.scale2 = FLT_MIN;
     p.page_log2 = 0, p.parts = nullptr, p.notes = nullptr;
     while ((1 << p.page_log2) < page) ++p.page_log2;
     c.k = k_cache, c.v = v_cache, c.k_p = k_page, c.k_h = k_head, c.v_p = v_page, c.v_h = v_head, c.tokens = tokens, c.d = d, c.dtype = dtype, c.page = page, c.sms = sm_count();
@@ -124,16 +61,5 @@ extern "C" int kyb_paged_attention(const void* q, int64_t q_t, int64_t q_h, cons
     KYB_REQUIRE(!need || ((uintptr_t)ws & 15) == 0, "the workspace must be 16-byte aligned");
     const int64_t rows = std::max<int64_t>(max_q, 1) * p.group;
     if (rows <= KYB_DECODE_ROWS) return kyb_attn_decode(c, (int)rows, ws);
-    kyb::SimpleParams sp;
-    sp.a = p, sp.k = (const uint8_t*)k_cache, sp.v = (const uint8_t*)v_cache, sp.k_p = k_page, sp.k_h = k_head, sp.v_p = v_page, sp.v_h = v_head;
-    const dim3 grid((unsigned)tokens, (unsigned)hq);
-    cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == 1) {
-        if (d == 64) kyb::paged_attn_simple_kernel<__half, 64><<<grid, 128, 0, st>>>(sp);
-        else kyb::paged_attn_simple_kernel<__half, 128><<<grid, 128, 0, st>>>(sp);
-    } else {
-        if (d == 64) kyb::paged_attn_simple_kernel<__nv_bfloat16, 64><<<grid, 128, 0, st>>>(sp);
-        else kyb::paged_attn_simple_kernel<__nv_bfloat16, 128><<<grid, 128, 0, st>>>(sp);
-    }
-    return kyb_launch_check("paged_attention");
+    return kyb_attn_prefill(c, ws);
 }

@@ -104,6 +104,8 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* tm,
                  "r"(page), "r"(bar)
                  : "memory");
 }
+// a wait whose answer is the warp's: what follows stands warp-wide instructions that a part of the warp must not meet alone
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_fast(bar, parity)); }
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -162,5 +164,7 @@ struct KybAttnCall {
 constexpr int KYB_DECODE_ROWS = 16;
 size_t kyb_attn_decode_scratch(int d, int rows, int sms);
 int kyb_attn_decode(KybAttnCall& c, int rows, void* ws);
+size_t kyb_attn_prefill_scratch(int d, int group, int sms);
+int kyb_attn_prefill(KybAttnCall& c, void* ws);
 // second launch: adds the parts of the items that were cut (ctas runs, blocks of `block` rows)
 int kyb_attn_join(const KybAttnCall& c, int ctas, int block);

@@ -33,7 +33,6 @@ __device__ __forceinline__ uint32_t turn8x8(uint32_t v) {
     return d;
 }
 __device__ __forceinline__ void consumer_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_fast(bar, parity)); }
 
 template <int D, int NT>
 struct DecodeShape {
@@ -343,52 +342,61 @@ __global__ void __launch_bounds__(DC_THREADS, 2) paged_attn_decode_kernel(const 
     if (failed) atomicExch(p.status, KYB_DEV_TIMEOUT_ATTN);
 }
 
-// The parts of the items that begin in run blockIdx.x and end in a later one: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i, in the order of the runs. One block
-// per (run, row); a thread holds one value of the row.
+// The parts of the items that begin in run blockIdx.x and end in a later one: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i, in the order of the runs. A warp per
+// row, a lane holds D / 32 of its values; the parts' maxima and sums are read 32 at a time.
+constexpr int JOIN_ROWS = 8;
 template <typename T, int D>
-__global__ void __launch_bounds__(D) paged_attn_join_kernel(const AttnParams p, const int ctas, const int block) {
-    __shared__ float weight[512];
-    __shared__ float top_s[D / 32], sum_s[D / 32];
+__global__ void __launch_bounds__(32 * JOIN_ROWS) paged_attn_join_kernel(const AttnParams p, const int ctas, const int block) {
+    constexpr int E = D / 32;
     pdl_wait();
-    const int first = blockIdx.x, rr = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int first = blockIdx.x, lane = threadIdx.x & 31, rr = blockIdx.y * JOIN_ROWS + (threadIdx.x >> 5);
     const int4 note = p.notes[first];
-    if (!(note.w & NOTE_BEGINS)) return;
+    if (!(note.w & NOTE_BEGINS) || rr >= block) return;
     int row_base;
     const int tokens = request_rows(p, note.x, row_base), row = note.y * block + rr, tok = row / p.group;
     if (tok >= tokens) return;
     const size_t size = (size_t)block * (D + 2);
-    int n = 1;                                                               // parts
-    while (first + n < ctas && !(p.notes[first + n].w & NOTE_ENDS)) ++n;
-    ++n;
-    auto part = [&](int i) { return p.parts + ((size_t)(first + i) * 2 + (i == 0)) * size; };
+    int n = 1;                                                               // parts: up to the run that ends the item
+    for (bool more = true; more && first + n < ctas;) {
+        const int i = first + n + lane;
+        const uint32_t ends = __ballot_sync(0xffffffffu, i >= ctas || (p.notes[i].w & NOTE_ENDS));
+        n += ends ? __ffs(ends) : 32, more = !ends;
+    }
+    n = min(n, ctas - first);
+    const float* const head = p.parts + ((size_t)first * 2 + 1) * size, * const rest = p.parts + (size_t)(first + 1) * 2 * size;   // part 0, and part i at rest + 2 (i - 1) size
     float top = -INFINITY;
-    for (int i = tid; i < n; i += D) top = fmaxf(top, part(i)[block * D + rr]);
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, (i ? rest + (size_t)(i - 1) * 2 * size : head)[(size_t)block * D + rr]);
 #pragma unroll
     for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    if (lane == 0) top_s[warp] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < D / 32; ++w) top = fmaxf(top, top_s[w]);
-    float sum = 0.f;
-    for (int i = tid; i < n; i += D) {
-        const float m = part(i)[block * D + rr], f = m == -INFINITY ? 0.f : exp2f(m - top);
-        weight[i] = f;
-        sum += f * part(i)[block * D + block + rr];
+    float o[E] = {}, sum = 0.f;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        const int i = i0 + lane;
+        float w = 0.f;
+        if (i < n) {
+            const float* const x = (i ? rest + (size_t)(i - 1) * 2 * size : head) + (size_t)block * D + rr;
+            w = x[0] == -INFINITY ? 0.f : exp2f(x[0] - top);
+            sum += w * x[block];
+        }
+        const int k = min(32, n - i0);
+#pragma unroll 4
+        for (int j = 0; j < k; ++j) {
+            const float* const x = (i0 + j ? rest + (size_t)(i0 + j - 1) * 2 * size : head) + (size_t)rr * D + lane * E;
+            const float wj = __shfl_sync(0xffffffffu, w, j);
+            if constexpr (E == 4) {
+                const float4 v = *reinterpret_cast<const float4*>(x);
+                o[0] += wj * v.x, o[1] += wj * v.y, o[2] += wj * v.z, o[3] += wj * v.w;
+            } else {
+                const float2 v = *reinterpret_cast<const float2*>(x);
+                o[0] += wj * v.x, o[1] += wj * v.y;
+            }
+        }
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (lane == 0) sum_s[warp] = sum;
-    __syncthreads();
-    sum = 0.f;
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    T* const out = reinterpret_cast<T*>(p.o) + (int64_t)(row_base + tok) * p.o_t + (int64_t)(note.z * p.group + row - tok * p.group) * p.o_h + lane * E;
 #pragma unroll
-    for (int w = 0; w < D / 32; ++w) sum += sum_s[w];
-    float o = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) o += weight[i] * part(i)[rr * D + tid];
-    o = sum > 0.f ? o / sum : 0.f;
-    T* const out = reinterpret_cast<T*>(p.o) + (int64_t)(row_base + tok) * p.o_t + (int64_t)(note.z * p.group + row - tok * p.group) * p.o_h;
-    const uint32_t w = pack2<T>(o, o);
-    reinterpret_cast<uint16_t*>(out)[tid] = (uint16_t)w;
+    for (int e = 0; e < E; e += 2) reinterpret_cast<uint32_t*>(out)[e / 2] = pack2<T>(o[e] * inv, o[e + 1] * inv);
 }
 
 }  // namespace kyb
@@ -431,7 +439,7 @@ int kyb_attn_decode(KybAttnCall& c, int rows, void* ws) {
 
 int kyb_attn_join(const KybAttnCall& c, int ctas, int block) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ctas, (unsigned)block), cfg.blockDim = dim3((unsigned)c.d), cfg.stream = c.st;
+    cfg.gridDim = dim3((unsigned)ctas, (unsigned)((block + kyb::JOIN_ROWS - 1) / kyb::JOIN_ROWS)), cfg.blockDim = dim3(32 * kyb::JOIN_ROWS), cfg.stream = c.st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;

@@ -1,0 +1,537 @@
+// Attention over a paged cache for many rows a request and head (chunks of prompts, whole prompts), bound by the tensor cores and the exponentials.
+//
+// One persistent CTA an SM. A row block is two query tiles of 128 / G tokens (G query heads each: up to 128 rows, so the heads of a group share every key). Warps:
+//   0-3, 4-7   softmax of the first and the second query tile, one row a thread
+//   8          producer: query tiles, and a ring of 128-key tiles of K and V by tiled copies (one per page piece and half of the values)
+//   9          tcgen05.mma issuer (10 and 11 are idle: registers move between groups of four warps, from these four to the softmax)
+// Tensor memory: S0 | S1 | O0 | O1, 128 columns each; the weights P (16 bits) take the place of their scores S. S = Q K^T with both operands in shared memory; O += P V with
+// P in tensor memory and V as it lies in the cache (MN-major operand). The issuer's order S0(j+1) behind O0(j), S1(j+1) behind O1(j) keeps the tensor cores busy
+// with one query tile while the softmax of the other runs. A row's reference maximum moves only when a score passes it by 2^8, so O is rescaled (by the softmax warps
+// themselves, in tensor memory) a few times per row at most; sums are of the unrounded weights, in 32 bits.
+// Keys that a row does not see are masked by selection in the tiles at the borders; values in places that no row of the block sees are cleared in shared memory, since such
+// places may hold anything and 0 times NaN is NaN.
+#include <algorithm>
+
+#include "paged_attn.cuh"
+
+namespace kyb {
+
+constexpr int PF_TILE = 128, PF_THREADS = 384;
+
+template <int D>
+struct PrefillShape {
+    static constexpr uint32_t HALVES = D / 64, HALF = 128 * 128, TILE = HALVES * HALF;       // a tile of 128 rows: halves of 64 values, 128-byte rows
+    static constexpr int SLOTS = D == 128 ? 5 : 10;
+    static constexpr uint32_t OFF_KV = 2 * TILE, OFF_BAR = OFF_KV + SLOTS * TILE, OFF_CUR = OFF_BAR + 16 * SLOTS + 64, SMEM = OFF_CUR + 8 * sizeof(Cursor);
+};
+
+__device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+                 "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld_16(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+                   "=r"(v[14]), "=r"(v[15])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait_all() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// O[tmem] (+)= P[tmem] * V[smem], issued by one thread
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// MN-major operand (V: [key][value], 128-byte swizzle): 64-value column blocks HALF bytes apart (leading offset), groups of 8 keys 1024 bytes apart (stride offset)
+__device__ __forceinline__ uint64_t umma_desc_mn128(uint32_t smem_addr, uint32_t half) {
+    return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(half >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// The bounded wait of this kernel, inline: a call would bind the caller to a calling convention's registers, which do not go with registers that move between warps.
+__device__ __forceinline__ bool wait_here(uint32_t bar, uint32_t parity) {
+    uint32_t ok = 0;
+#pragma unroll 1
+    for (uint32_t i = 0; i < (1u << 22); ++i) {
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) break;
+        if (i > 64) __nanosleep(64);
+    }
+    return __all_sync(0xffffffffu, ok);
+}
+
+// smallest i with v[i] > x (v not decreasing, v[n - 1] > x)
+__device__ __forceinline__ int first_end_above(const int* v, int n, int x) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (v[mid] > x) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+}
+
+struct RunFinder {
+    int tokens[PF_THREADS], kv[PF_THREADS], blocks_end[PF_THREADS];
+    unsigned long long tiles[PF_THREADS];
+    long long sums[PF_THREADS / 32];
+    Cursor run;
+    long long at;
+    int request;
+};
+__device__ __forceinline__ long long scan_block(long long v, long long* sums, long long& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += x;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = v;
+    __syncthreads();
+    total = 0;
+    for (int w = 0; w < PF_THREADS / 32; ++w) {
+        if (w < warp) v += sums[w];
+        total += sums[w];
+    }
+    return v;
+}
+// tiles of up to PF_THREADS requests from r0 on, of all heads: the row blocks of all of them are shared among the threads
+__device__ __forceinline__ long long count_chunk(const AttnParams& p, int block, int r0, RunFinder& f, long long& end) {
+    const int tid = threadIdx.x, n = min(PF_THREADS, p.batch - r0);
+    int nb = 0;
+    __syncthreads();
+    if (tid < n) {
+        int base;
+        f.tokens[tid] = request_rows(p, r0 + tid, base), f.kv[tid] = request_keys(p, r0 + tid);
+        nb = row_blocks(p, f.tokens[tid], block);
+    }
+    f.tiles[tid] = 0;
+    long long all;
+    f.blocks_end[tid] = (int)scan_block(nb, f.sums, all);
+    __syncthreads();
+    for (int i = tid; i < (int)all; i += PF_THREADS) {
+        const int r = first_end_above(f.blocks_end, n, i), rb = i - (r ? f.blocks_end[r - 1] : 0);
+        atomicAdd(&f.tiles[r], (unsigned long long)key_span(p, f.tokens[r], f.kv[r], block, rb, PF_TILE).n * p.hkv);       // whole numbers: the order does not matter
+    }
+    __syncthreads();
+    long long total;
+    end = scan_block((long long)f.tiles[tid], f.sums, total);
+    return total;
+}
+// The run of tiles of CTA blockIdx.x, into f.run
+__device__ __forceinline__ void find_run_wide(const AttnParams& p, int block, RunFinder& f) {
+    const int tid = threadIdx.x;
+    long long total = 0, end = 0, mine = 0;
+    for (int r0 = 0; r0 < p.batch; r0 += PF_THREADS) mine = count_chunk(p, block, r0, f, end), total += mine;
+    const long long ctas = min((long long)gridDim.x, total), c = blockIdx.x;
+    const long long u0 = c < ctas ? total * c / ctas : 0, u1 = c < ctas ? total * (c + 1) / ctas : 0;
+    if (tid == 0) f.run.left = u1 - u0;
+    __syncthreads();
+    if (u1 == u0) return;
+    long long before = 0;
+    for (int r0 = 0; r0 < p.batch && before <= u0; r0 += PF_THREADS) {
+        if (p.batch > PF_THREADS) mine = count_chunk(p, block, r0, f, end);
+        const long long e = before + end, n = (long long)f.tiles[tid];
+        if (n && u0 >= e - n && u0 < e) f.request = r0 + tid, f.at = u0 - (e - n);
+        before += mine;
+        __syncthreads();
+    }
+    const int r = f.request;
+    const long long at = f.at;
+    int base;
+    const int tokens = request_rows(p, r, base), kv = request_keys(p, r), nb = row_blocks(p, tokens, block);
+    before = 0;
+    for (int b0 = 0; b0 < nb && before <= at; b0 += PF_THREADS) {
+        const int rb = b0 + tid, one = rb < nb ? key_span(p, tokens, kv, block, rb, PF_TILE).n : 0;
+        long long all;
+        const long long e = before + scan_block((long long)one * p.hkv, f.sums, all), n = (long long)one * p.hkv;
+        if (n && at >= e - n && at < e) {
+            Cursor& k = f.run;
+            k.r = r, k.rb = rb;
+            k.load(p, block, PF_TILE);
+            k.h = (int)((at - (e - n)) / one), k.at = (int)((at - (e - n)) % one);
+        }
+        before += all;
+        __syncthreads();
+    }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(PF_THREADS, 1) paged_attn_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                                           const __grid_constant__ CUtensorMap map_v, const AttnParams p, const int qtoks) {
+    using S = PrefillShape<D>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u, kv0 = smem0 + S::OFF_KV;
+    const uint32_t full0 = smem0 + S::OFF_BAR, empty0 = full0 + 8 * S::SLOTS, qfull = empty0 + 8 * S::SLOTS, qempty = qfull + 8, sfull0 = qfull + 16, pfull0 = qfull + 32, tmem_slot = qfull + 48;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int qrows = qtoks * p.group, block = 2 * qrows;                    // rows of a query tile, of a row block
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::SLOTS; ++s) mbar_init_a(full0 + 8 * s, 1), mbar_init_a(empty0 + 8 * s, 1);
+        mbar_init_a(qfull, 1), mbar_init_a(qempty, 1);
+        for (int w = 0; w < 2; ++w) mbar_init_a(sfull0 + 8 * w, 1), mbar_init_a(pfull0 + 8 * w, 4);
+        mbar_fence_init();
+        prefetch_tmap(&map_q), prefetch_tmap(&map_k), prefetch_tmap(&map_v);
+    }
+    if (warp == 9) tmem_alloc(tmem_slot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = lds32(tmem_slot);
+    RunFinder& finder = *reinterpret_cast<RunFinder*>(smem_raw + (kv0 - smem_u32(smem_raw)));       // where the ring will be
+    find_run_wide(p, block, finder);
+    __syncthreads();
+    const Cursor c0 = finder.run;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+    pdl_launch_dependents();
+    bool failed = false;
+
+    // registers move from the producer's group of four warps to the softmax groups: 72 + 2 x 216 = 3 x 168, what the block was launched with
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+      if (warp == 8) {
+        // ---- producer: lane i looks up the page of the run's piece `base + i`; lanes issue the copies of a tile's pieces and halves
+        const int page = 1 << p.page_log2, piece = min(page, PF_TILE), piece_log2 = min(p.page_log2, 7), pieces = PF_TILE >> piece_log2, per_load = 32 / pieces;
+        Cursor c = c0;
+        int s = 0, issued = 0;
+        uint32_t parity = 1, qparity = 1;
+        while (c.left > 0) {
+            const int run = (int)min((long long)(c.s.n - c.at), c.left);
+            const int tiles_q = c.s.rows > qrows ? 2 : 1;
+            if (!failed && !wait_here(qempty, qparity)) failed = true;
+            qparity ^= 1u;
+            if (!failed) {
+                if (lane == 0) mbar_expect_tx_a(qfull, (uint32_t)tiles_q * S::HALVES * (uint32_t)qrows * 128u);
+                __syncwarp();
+                if (lane < tiles_q * (int)S::HALVES) {
+                    const int w = lane / (int)S::HALVES, half = lane % (int)S::HALVES;
+                    tma_load_5d(smem0 + w * S::TILE + half * S::HALF, &map_q, 0, half, 0, c.h, c.row_base + c.s.row0 / p.group + w * qtoks, qfull);
+                }
+            }
+            auto lookup = [&](int i) {                                       // the pages of the pieces of tiles i, i + 1, ...
+                const int tl = i + lane / pieces, key = tl < c.s.n ? c.s.tile(tl) * PF_TILE + ((lane & (pieces - 1)) << piece_log2) : p.cap;
+                const bool seen = key < c.s.end && (key + piece > c.s.lo || key < p.sinks);
+                int id = seen ? p.table[c.r * p.ld_table + (key >> p.page_log2)] : p.pages;      // a piece that no row sees is read as if it lay behind the cache: zeros
+                return (unsigned)id >= (unsigned)p.pages ? p.pages : id;
+            };
+            int base = c.at, ids = lookup(base), ids_next = lookup(base + per_load);
+            for (int i = c.at; i < c.at + run && !failed; ++i) {
+                if (i - base == per_load) base = i, ids = ids_next, ids_next = lookup(base + per_load);
+                const int j = lane / (int)S::HALVES, half = lane % (int)S::HALVES;
+                const int id = __shfl_sync(0xffffffffu, ids, (i - base) * pieces + (j & (pieces - 1)));
+                const int y = (c.s.tile(i) * PF_TILE + (j << piece_log2)) & (page - 1);
+#pragma unroll
+                for (int kv = 0; kv < 2 && !failed; ++kv) {
+                    if (!wait_here(empty0 + 8 * s, parity)) {
+                        failed = true;
+                        break;
+                    }
+                    if (lane == 0) mbar_expect_tx_a(full0 + 8 * s, S::TILE);
+                    __syncwarp();
+                    if (j < pieces) tma_load_5d(kv0 + s * S::TILE + half * S::HALF + j * (piece * 128), kv ? &map_v : &map_k, 0, y, half, c.h, id, full0 + 8 * s);
+                    ++issued;
+                    if (++s == S::SLOTS) s = 0, parity ^= 1u;
+                }
+            }
+            c.left -= run, c.at += run;
+            if (c.at == c.s.n) c.next(p, block, PF_TILE);
+        }
+        if (failed)                                                          // copies in flight end before the block does
+            for (int k = 0; k < min(issued, S::SLOTS); ++k) {
+                const int at = issued - 1 - k;
+                wait_here(full0 + 8 * (at % S::SLOTS), (uint32_t)(at / S::SLOTS) & 1u);
+            }
+      } else if (warp == 9) {
+        // ---- issuer
+        Cursor c = c0;
+        constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
+        constexpr uint32_t idesc_s = umma_idesc_f16(128, 128) | fmt, idesc_o = umma_idesc_f16(128, D) | fmt | (1u << 16);      // V: MN-major
+        int s = 0;
+        uint32_t parity = 0, qparity = 0, pparity0 = 0, pparity1 = 0;
+        auto wait = [&](uint32_t bar, uint32_t par) {
+            if (!failed && !wait_here(bar, par)) failed = true;
+            tc_fence_after();
+        };
+        auto scores = [&](int w, int slot) {                                 // S_w = Q_w K^T
+#pragma unroll
+            for (int h = 0; h < (int)S::HALVES; ++h) {
+                const uint64_t a = umma_desc_sw128(smem0 + w * S::TILE + h * S::HALF), b = umma_desc_sw128(kv0 + slot * S::TILE + h * S::HALF);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) umma_f16(tmem + 128 * w, a + 2 * k, b + 2 * k, idesc_s, (h | k) != 0);
+            }
+        };
+        auto values = [&](int w, int slot, bool first) {                     // O_w += P_w V
+            const uint64_t b = umma_desc_mn128(kv0 + slot * S::TILE, S::HALF);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) umma_f16_ts(tmem + 256 + 128 * w, tmem + 128 * w + 8 * k, b + 128 * k, idesc_o, !first || k);
+        };
+        while (c.left > 0) {
+            const int run = (int)min((long long)(c.s.n - c.at), c.left);
+            const bool two = c.s.rows > qrows;
+            wait(qfull, qparity);
+            qparity ^= 1u;
+            int slot_k = s;
+            wait(full0 + 8 * slot_k, parity);
+            if (++s == S::SLOTS) s = 0, parity ^= 1u;
+            if (!failed && elect_one()) {
+                scores(0, slot_k);
+                umma_commit(sfull0);
+                if (two) scores(1, slot_k), umma_commit(sfull0 + 8);
+                umma_commit(empty0 + 8 * slot_k);
+                if (run == 1) umma_commit(qempty);
+            }
+            __syncwarp();
+            for (int i = 0; i < run; ++i) {
+                const int slot_v = s;
+                wait(full0 + 8 * slot_v, parity);
+                if (++s == S::SLOTS) s = 0, parity ^= 1u;
+                const int key0 = c.s.tile(c.at + i) * PF_TILE;
+                if (!(key0 + PF_TILE <= c.s.end && (key0 >= c.s.lo || key0 + PF_TILE <= p.sinks)) && !failed) {
+                    // places that no row sees: their values become 0
+                    for (int x = lane; x < PF_TILE * (int)S::HALVES * 8; x += 32) {
+                        const int key = x / ((int)S::HALVES * 8), ch = x % ((int)S::HALVES * 8);
+                        if (!c.s.alive(key0 + key, p.sinks))
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(kv0 + slot_v * S::TILE + (ch >> 3) * S::HALF + key * 128 + (ch & 7) * 16), "r"(0) : "memory");
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+                const bool more = i + 1 < run;
+                slot_k = s;
+                wait(pfull0, pparity0);
+                pparity0 ^= 1u;
+                if (!failed && elect_one()) values(0, slot_v, i == 0);
+                __syncwarp();
+                if (more) {
+                    wait(full0 + 8 * slot_k, parity);
+                    if (++s == S::SLOTS) s = 0, parity ^= 1u;
+                }
+                if (!failed && elect_one()) {
+                    if (more) scores(0, slot_k);
+                    umma_commit(sfull0);                                     // S0 of the next tile is there, O0 of this one too
+                }
+                __syncwarp();
+                if (two) {
+                    wait(pfull0 + 8, pparity1);
+                    pparity1 ^= 1u;
+                    if (!failed && elect_one()) {
+                        values(1, slot_v, i == 0);
+                        umma_commit(empty0 + 8 * slot_v);
+                        if (more) scores(1, slot_k);
+                        umma_commit(sfull0 + 8);
+                        if (more) umma_commit(empty0 + 8 * slot_k);
+                        if (i + 2 == run) umma_commit(qempty);
+                    }
+                } else if (!failed && elect_one()) {
+                    umma_commit(empty0 + 8 * slot_v);
+                    if (more) umma_commit(empty0 + 8 * slot_k);
+                    if (i + 2 == run) umma_commit(qempty);
+                }
+                __syncwarp();
+            }
+            c.left -= run, c.at += run;
+            if (c.at == c.s.n) c.next(p, block, PF_TILE);
+        }
+      }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        // ---- softmax: one row a thread
+        const int w = warp >> 2, rl = (warp & 3) * 32 + lane;
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lane_base + 128u * w, to = ts + 256u, sfull = sfull0 + 8 * w, pfull = pfull0 + 8 * w;
+        const float scale2 = fabsf(p.scale2);
+        const bool flip = p.scale2 < 0.f;
+        uint32_t sparity = 0;
+        int flags = 0;
+        // the warp's place in its run lies in shared memory: a row's 128 scores take the registers
+        Cursor& c = *reinterpret_cast<Cursor*>(smem_raw + (smem0 - smem_u32(smem_raw)) + S::OFF_CUR + warp * sizeof(Cursor));
+        if (lane == 0) c = c0;
+        __syncwarp();
+        while (c.left > 0) {
+            const int from = c.at, run = (int)min((long long)(c.s.n - from), c.left);
+            const int row = w * qrows + rl;                                  // row of the block
+            const bool on = rl < qrows && row < c.s.rows;
+            float m = -INFINITY, l = 0.f;
+            if (w == 0 || c.s.rows > qrows) {                                // the second tile may be empty: then nothing of it is issued
+                const int pos = on ? c.kv - c.tokens + (c.s.row0 + row) / p.group : -1, sink_tiles = c.s.sink_tiles, main_tile = c.s.main_tile - sink_tiles;
+                // tiles from key plain_lo to plain_hi need no masks for any row of the query tile
+                const int plain_hi = min(c.s.first + w * qtoks + 1, p.cap) - PF_TILE, plain_lo = p.window ? min(c.s.last, c.s.first + (w + 1) * qtoks - 1) - p.window + 1 : 0;
+                for (int i = 0; i < run; ++i) {
+                    if (!failed && !wait_here(sfull, sparity)) failed = true;
+                    sparity ^= 1u;
+                    tc_fence_after();
+                    uint32_t v[4][32];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) tmem_ld_32x32(ts + 32 * q, v[q]);
+                    tmem_ld_wait();
+                    const int key0 = (from + i + (from + i < sink_tiles ? 0 : main_tile)) * PF_TILE;
+                    if (flip)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) v[q][e] ^= 0x80000000u;
+                    if (key0 > plain_hi || key0 < plain_lo) {
+                        const int hi = min(pos, p.cap - 1) - key0, lo = p.window ? pos - p.window + 1 - key0 : -1, sk = p.sinks - key0;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) {
+                                const int col = 32 * q + e;
+                                if (!(col <= hi && (col >= lo || col < sk))) v[q][e] = 0xff800000u;
+                            }
+                    }
+                    float t[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        float a = __uint_as_float(v[q][0]);
+#pragma unroll
+                        for (int e = 1; e < 32; ++e) a = fmaxf(a, __uint_as_float(v[q][e]));
+                        t[q] = a;
+                    }
+                    const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * scale2;
+                    const bool over = top > m + 8.f;                         // false where nothing is seen yet (-inf on both sides)
+                    if (__any_sync(0xffffffffu, over)) {
+                        const float f = !over ? 1.f : m == -INFINITY ? 0.f : exp2_fast(m - top);
+                        if (over) m = top;
+                        l *= f;
+                        if (i) {
+#pragma unroll 1
+                            for (int q = 0; q < D; q += 16) {
+                                uint32_t x[16];
+                                tmem_ld_16(to + q, x);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+                                tmem_st_16(to + q, x);
+                            }
+                        }
+                    }
+                    const float m0 = m == -INFINITY ? 0.f : m;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            const float a = exp2_fast(fmaf(__uint_as_float(v[q][e]), scale2, -m0)), b = exp2_fast(fmaf(__uint_as_float(v[q][e + 1]), scale2, -m0));
+                            sum[(e >> 1) & 3] += a + b;
+                            pk[e / 2] = pack2<T>(a, b);
+                        }
+                        tmem_st_16(ts + 16 * q, pk);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tmem_st_wait_all();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_a(pfull);
+                }
+                if (!failed && !wait_here(sfull, sparity)) failed = true;    // the last O
+                sparity ^= 1u;
+                tc_fence_after();
+                const float inv = l > 0.f ? 1.f / l : 0.f;
+                const bool whole = from == 0 && run == c.s.n;
+                const int tok = (c.s.row0 + row) / p.group;
+                T* const out = reinterpret_cast<T*>(p.o) + (int64_t)(c.row_base + (on ? tok : 0)) * p.o_t + (int64_t)(c.h * p.group + (on ? c.s.row0 + row - tok * p.group : 0)) * p.o_h;
+                float* const part = p.parts + ((size_t)blockIdx.x * 2 + (from == 0)) * ((size_t)block * (D + 2)) + (size_t)row * D;
+#pragma unroll 1
+                for (int q = 0; q < D; q += 32) {
+                    uint32_t x[32];
+                    tmem_ld_32x32(to + q, x);
+                    tmem_ld_wait();
+                    if (!on || failed) continue;
+                    if (whole) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            uint4 y;
+                            y.x = pack2<T>(__uint_as_float(x[e]) * inv, __uint_as_float(x[e + 1]) * inv), y.y = pack2<T>(__uint_as_float(x[e + 2]) * inv, __uint_as_float(x[e + 3]) * inv);
+                            y.z = pack2<T>(__uint_as_float(x[e + 4]) * inv, __uint_as_float(x[e + 5]) * inv), y.w = pack2<T>(__uint_as_float(x[e + 6]) * inv, __uint_as_float(x[e + 7]) * inv);
+                            *reinterpret_cast<uint4*>(out + q + e) = y;
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            *reinterpret_cast<float4*>(part + q + e) = make_float4(__uint_as_float(x[e]), __uint_as_float(x[e + 1]), __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+                    }
+                }
+                if (on && !whole && !failed) {
+                    float* const ml = part - (size_t)row * D + (size_t)block * D + row;
+                    ml[0] = m, ml[block] = l;
+                }
+                tc_fence_before();
+            }
+            __syncwarp();
+            if (lane == 0) {
+                if (from != 0 || run != c.s.n) flags |= from == 0 ? NOTE_BEGINS : NOTE_CONTINUES | (from + run == c.s.n ? NOTE_ENDS : 0);
+                c.left -= run, c.at += run;
+                if (warp == 0 && c.left == 0) p.notes[blockIdx.x] = make_int4(c.r, c.s.row0 / block, c.h, flags);
+                if (c.at == c.s.n) c.next(p, block, PF_TILE);
+            }
+            __syncwarp();
+        }
+        if (c0.left == 0 && threadIdx.x == 0) p.notes[blockIdx.x] = make_int4(0, 0, 0, 0);
+    }
+    if (failed) atomicExch(p.status, KYB_DEV_TIMEOUT_ATTN);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+}  // namespace kyb
+
+namespace {
+
+// queries [tokens][kv heads][group][d]: {64 values, half, head of the group, kv head, token}, boxes of all heads of a group and `qtoks` tokens
+int make_query_map(CUtensorMap* tm, const KybAttnCall& c, int qtoks) {
+    kyb_encode_tiled_fn enc = kyb_get_encode_tiled();
+    if (!enc) {
+        kyb_set_error("cuTensorMapEncodeTiled is not available from this driver");
+        return KYB_ECUDA;
+    }
+    const kyb::AttnParams& p = c.p;
+    const int64_t head = p.hq == 1 ? c.d : p.q_h, token = c.tokens == 1 ? (int64_t)c.d * p.hq : p.q_t;       // the stride of a dimension of one is never used: any valid one
+    const cuuint64_t dims[5] = {64, (cuuint64_t)(c.d / 64), (cuuint64_t)p.group, (cuuint64_t)p.hkv, (cuuint64_t)c.tokens};
+    const cuuint64_t strides[4] = {128, (cuuint64_t)head * 2, (cuuint64_t)head * 2 * (cuuint64_t)p.group, (cuuint64_t)token * 2};
+    const cuuint32_t box[5] = {64, 1, (cuuint32_t)p.group, 1, (cuuint32_t)qtoks}, estr[5] = {1, 1, 1, 1, 1};
+    const CUresult r = enc(tm, c.dtype == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<uint8_t*>(p.q), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        kyb_set_error("cuTensorMapEncodeTiled failed with CUresult %d (queries %p: %lld tokens, %d x %d heads of %d, strides %lld, %lld)", (int)r, (const void*)p.q, (long long)c.tokens, p.hkv,
+                      p.group, c.d, (long long)token, (long long)head);
+        return KYB_ECUDA;
+    }
+    return KYB_OK;
+}
+
+template <typename T, int D>
+int launch_prefill(KybAttnCall& c, void* ws) {
+    using S = kyb::PrefillShape<D>;
+    auto kern = kyb::paged_attn_prefill_kernel<T, D>;
+    if (int rc = kyb_allow_smem((const void*)kern)) return rc;
+    const int ctas = c.sms, piece = std::min(c.page, kyb::PF_TILE), qtoks = 128 / c.p.group;
+    CUtensorMap mq, mk, mv;
+    if (int rc = make_query_map(&mq, c, qtoks)) return rc;
+    if (int rc = kyb_make_cache_map(&mk, c.k, c.dtype, c.p.pages, c.p.hkv, c.page, D, c.k_p, c.k_h, piece, 1)) return rc;
+    if (int rc = kyb_make_cache_map(&mv, c.v, c.dtype, c.p.pages, c.p.hkv, c.page, D, c.v_p, c.v_h, piece, 1)) return rc;
+    c.p.notes = (int4*)ws, c.p.parts = (float*)((char*)ws + (size_t)ctas * sizeof(int4));
+    kern<<<(unsigned)ctas, kyb::PF_THREADS, S::SMEM + 1024, c.st>>>(mq, mk, mv, c.p, qtoks);
+    if (int rc = kyb_launch_check("paged_attn_prefill")) return rc;
+    return kyb_attn_join(c, ctas, 2 * qtoks * c.p.group);
+}
+
+}  // namespace
+
+size_t kyb_attn_prefill_scratch(int d, int group, int sms) {
+    const size_t block = 2 * (size_t)(128 / group) * (size_t)group;
+    return (size_t)sms * (sizeof(int4) + 2 * block * (d + 2) * sizeof(float));
+}
+
+int kyb_attn_prefill(KybAttnCall& c, void* ws) {
+    if (c.dtype == 1) return c.d == 64 ? launch_prefill<__half, 64>(c, ws) : launch_prefill<__half, 128>(c, ws);
+    return c.d == 64 ? launch_prefill<__nv_bfloat16, 64>(c, ws) : launch_prefill<__nv_bfloat16, 128>(c, ws);
+}
