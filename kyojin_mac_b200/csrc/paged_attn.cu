@@ -26,6 +26,7 @@ extern "C" int kyb_paged_attention(const void* q, int64_t q_t, int64_t q_h, cons
     KYB_REQUIRE(batch > 0 && batch < (1ll << 24) && tokens >= 0 && tokens < (1ll << 30) && max_q >= 0, "batch=%lld tokens=%lld max_q=%lld: out of range", (long long)batch, (long long)tokens,
                 (long long)max_q);
     KYB_REQUIRE(hkv > 0 && hq > 0 && hq % hkv == 0 && hq / hkv <= 128 && hkv <= 65535 && hq <= 65535, "heads %d / %d: query heads are a multiple (up to 128) of the key-value heads", hq, hkv);
+    KYB_REQUIRE(tokens * (hq / hkv) < (1ll << 30), "%lld tokens of %d heads a group: out of range", (long long)tokens, hq / hkv);
     KYB_REQUIRE(d == 64 || d == 128, "d=%d: heads of 64 or 128", d);
     KYB_REQUIRE(dtype == 1 || dtype == 2, "dtype=%d: 1 (fp16) or 2 (bf16)", dtype);
     KYB_REQUIRE(page >= 16 && page <= 256 && (page & (page - 1)) == 0 && pages > 0 && pages < (1ll << 31) - 1, "page=%d pages=%lld: a power of two from 16 to 256, at least one page", page,
@@ -48,7 +49,7 @@ extern "C" int kyb_paged_attention(const void* q, int64_t q_t, int64_t q_h, cons
     p.window = (int)std::min<int64_t>(window, 1 << 30), p.sinks = (int)std::min<int64_t>(sinks, 1 << 30), p.scale2 = scale * 1.4426950408889634f, p.status = status;
     // a hidden score is -inf and stays so times the scale: 0 would make it NaN, the smallest normal number gives the same weights
     if (!(p.scale2 >= FLT_MIN || p.scale2 <= -FLT_MIN)) p.scale2 = FLT_MIN;
-    p.page_log2 = 0, p.parts = nullptr, p.notes = nullptr;
+    p.page_log2 = 0, p.block_tokens = 0, p.parts = nullptr, p.notes = nullptr;
     while ((1 << p.page_log2) < page) ++p.page_log2;
     c.k = k_cache, c.v = v_cache, c.k_p = k_page, c.k_h = k_head, c.v_p = v_page, c.v_h = v_head, c.tokens = tokens, c.d = d, c.dtype = dtype, c.page = page, c.sms = sm_count();
     c.st = (cudaStream_t)stream;

@@ -3,7 +3,7 @@
 //
 // Rows: the (token, query head) pairs of one request and one key-value head, token by token, G = hq / hkv rows a token: all of them read the same keys. A row block
 // is `block` consecutive ones. An item is (request, row block, key-value head); its work is cut along the keys into tiles of `tile` keys. The tiles of all items, in
-// order (request, then row block, then head), are dealt to the CTAs in equal contiguous runs, so ragged lengths and few long ones balance alike; an item that a run's
+// order (request, then row block, then head), are dealt to the CTAs in contiguous runs of equal cost, so ragged lengths and few long ones balance alike; an item that a run's
 // border cuts leaves parts in the scratch, unnormalised and in 32 bits, which a second launch adds in their order. Nothing depends on timing.
 #pragma once
 
@@ -22,6 +22,7 @@ struct AttnParams {
     const int* cu_q;
     int64_t ld_table;
     int batch, tokens, hq, hkv, group, page_log2, pages, cap; // tokens: rows of q; cap: tokens that a row of the table can hold
+    int block_tokens;
     int window, sinks;                                        // window 0: none
     float scale2;                                             // scale log2(e)
     unsigned int* status;
@@ -42,10 +43,13 @@ struct KeySpan {
     __device__ __forceinline__ bool alive(int key, int sinks) const { return key < end && (key >= lo || key < sinks); }
 };
 
+// block: rows of a row block; p.block_tokens: its tokens when it is made of whole ones (no division by the group then), else 0
 __device__ __forceinline__ KeySpan key_span(const AttnParams& p, int tokens, int kv, int block, int rb, int tile) {
     KeySpan s;
     s.row0 = rb * block, s.rows = min(block, tokens * p.group - s.row0);
-    s.first = kv - tokens + s.row0 / p.group, s.last = kv - tokens + (s.row0 + s.rows - 1) / p.group;
+    if (p.block_tokens) s.first = rb * p.block_tokens, s.last = min(s.first + p.block_tokens, tokens) - 1;
+    else s.first = s.row0 / p.group, s.last = (s.row0 + s.rows - 1) / p.group;
+    s.first += kv - tokens, s.last += kv - tokens;
     s.end = max(0, min(s.last + 1, p.cap));
     s.lo = p.window ? max(0, s.first - p.window + 1) : 0;
     s.main_tile = s.lo / tile;
@@ -60,28 +64,44 @@ __device__ __forceinline__ int request_rows(const AttnParams& p, int r, int& bas
     return min(max(p.cu_q[r + 1], base), p.tokens) - base;
 }
 __device__ __forceinline__ int request_keys(const AttnParams& p, int r) { return min(max(p.kv_lens[r], 0), 1 << 30); }
-__device__ __forceinline__ int row_blocks(const AttnParams& p, int tokens, int block) { return (int)(((long long)max(0, tokens) * p.group + block - 1) / block); }
+__device__ __forceinline__ int row_blocks(const AttnParams& p, int tokens, int block) { return (tokens * p.group + block - 1) / block; }
 
-// Tiles of one key-value head of a request
-__device__ __forceinline__ long long request_tiles(const AttnParams& p, int r, int block, int tile, int lane = 0, int lanes = 1) {
-    int base;
-    const int tokens = request_rows(p, r, base), kv = request_keys(p, r), nb = row_blocks(p, tokens, block);
-    long long n = 0;
-    for (int b = lane; b < nb; b += lanes) n += key_span(p, tokens, kv, block, b, tile).n;
-    return n;
-}
+// The work is dealt in units: an item counts its tiles and OVER more, what beginning and ending it costs (measured, in tiles), in front of them. A border between runs that
+// falls into those, or so that SNAP tiles or fewer of the item would be left, moves to the item's begin or end: items are not cut for nothing.
+template <int OVER, int SNAP>
+struct Runs {
+    static __device__ __forceinline__ int units(const KeySpan& s) { return s.n + OVER; }
+    // a run that starts `x` units into an item: the tile it starts with (n: with the next item), and what changes in its number of units
+    static __device__ __forceinline__ int enter(const KeySpan& s, int x, long long& left) {
+        if (x > OVER && s.n + OVER - x <= SNAP) {
+            left -= s.n + OVER - x;
+            return s.n;
+        }
+        if (x <= OVER) {
+            left += x;
+            return 0;
+        }
+        return x - OVER;
+    }
+    // tiles of the item that a run with `left` units takes from tile `at` on (0: the run ends in front of it)
+    static __device__ __forceinline__ int take(const KeySpan& s, int at, long long left) {
+        const long long n = left - (at ? 0 : OVER);
+        return n <= 0 ? 0 : n + SNAP >= s.n - at ? s.n - at : (int)n;
+    }
+    static __device__ __forceinline__ int cost(int at, int taken) { return taken + (at ? 0 : OVER); }
+};
 
-// Where a CTA's run of tiles is: the item it starts in, and how many tiles it has
+// Where a CTA's run is
 struct Cursor {
     int r, rb, h, at;          // request, row block, head, next tile of the item
-    long long left;            // tiles left in the run
+    long long left;            // units left in the run
     int tokens, kv, blocks, row_base;
     KeySpan s;
     __device__ __forceinline__ void load(const AttnParams& p, int block, int tile) {
         tokens = request_rows(p, r, row_base), kv = request_keys(p, r), blocks = row_blocks(p, tokens, block);
         if (rb < blocks) s = key_span(p, tokens, kv, block, rb, tile);
     }
-    // behind an item: to the next one
+    // to the next item
     __device__ __forceinline__ void next(const AttnParams& p, int block, int tile) {
         at = 0;
         if (++h < p.hkv) return;
@@ -89,13 +109,19 @@ struct Cursor {
         while (rb >= blocks) {
             rb = 0;
             if (++r >= p.batch) {
-                left = 0;
+                r = p.batch - 1, left = 0;
                 return;
             }
             load(p, block, tile);
         }
         s = key_span(p, tokens, kv, block, rb, tile);
     }
+    // behind `taken` tiles
+    template <typename RUNS> __device__ __forceinline__ void advance(const AttnParams& p, int block, int tile, int taken) {
+        left -= RUNS::cost(at, taken), at += taken;
+        if (at == s.n) next(p, block, tile);
+    }
+    template <typename RUNS> __device__ __forceinline__ int run() const { return left > 0 ? RUNS::take(s, at, left) : 0; }
 };
 
 // 5-D copy of a piece of one page and head into shared memory: [half of the values][token][128 bytes], 128-byte swizzle

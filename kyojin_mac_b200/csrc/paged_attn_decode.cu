@@ -41,11 +41,20 @@ struct DecodeShape {
     static constexpr size_t PART = (size_t)ROWS * (D + 2);                                       // floats of a part
 };
 
+using DecodeRuns = Runs<1, 0>;
+__device__ __forceinline__ long long request_units(const AttnParams& p, int r, int block) {
+    int base;
+    const int tokens = request_rows(p, r, base), kv = request_keys(p, r), nb = row_blocks(p, tokens, block);
+    long long n = 0;
+    for (int b = 0; b < nb; ++b) n += DecodeRuns::units(key_span(p, tokens, kv, block, b, DC_TILE));
+    return n * p.hkv;
+}
+
 // First item and length of this CTA's run: every thread of the block takes part; the result is in *out (shared).
-__device__ __forceinline__ void find_run(const AttnParams& p, int block, int tile, Cursor* out, long long* sums, int threads) {
+__device__ __forceinline__ void find_run(const AttnParams& p, int block, Cursor* out, long long* sums, int threads) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = threads / 32;
     long long mine = 0;
-    for (int r = tid; r < p.batch; r += threads) mine += request_tiles(p, r, block, tile) * p.hkv;
+    for (int r = tid; r < p.batch; r += threads) mine += request_units(p, r, block);
     const long long first = mine;                                           // (this thread's only request when there are no more of them than threads)
 #pragma unroll
     for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
@@ -60,7 +69,7 @@ __device__ __forceinline__ void find_run(const AttnParams& p, int block, int til
     long long before = 0;
     for (int r0 = 0; r0 < p.batch && u1 > u0 && before <= u0; r0 += threads) {
         const int r = r0 + tid;
-        const long long n = r < p.batch ? (p.batch <= threads ? first : request_tiles(p, r, block, tile) * p.hkv) : 0;
+        const long long n = r < p.batch ? (p.batch <= threads ? first : request_units(p, r, block)) : 0;
         long long end = n;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -79,9 +88,11 @@ __device__ __forceinline__ void find_run(const AttnParams& p, int block, int til
             Cursor k;
             long long at = u0 - (end - n);
             k.r = r, k.rb = 0, k.left = u1 - u0;
-            k.load(p, block, tile);
-            while (at >= (long long)k.s.n * p.hkv) at -= (long long)k.s.n * p.hkv, ++k.rb, k.s = key_span(p, k.tokens, k.kv, block, k.rb, tile);
-            k.h = (int)(at / k.s.n), k.at = (int)(at % k.s.n);
+            k.load(p, block, DC_TILE);
+            while (at >= (long long)DecodeRuns::units(k.s) * p.hkv) at -= (long long)DecodeRuns::units(k.s) * p.hkv, ++k.rb, k.s = key_span(p, k.tokens, k.kv, block, k.rb, DC_TILE);
+            k.h = (int)(at / DecodeRuns::units(k.s));
+            k.at = DecodeRuns::enter(k.s, (int)(at % DecodeRuns::units(k.s)), k.left);
+            if (k.at == k.s.n) k.next(p, block, DC_TILE);
             *out = k;
         }
         before = all;
@@ -106,7 +117,7 @@ __global__ void __launch_bounds__(DC_THREADS, 2) paged_attn_decode_kernel(const 
         prefetch_tmap(&map_k);
         prefetch_tmap(&map_v);
     }
-    find_run(p, S::ROWS, DC_TILE, &start, sums, DC_THREADS);
+    find_run(p, S::ROWS, &start, sums, DC_THREADS);
     Cursor c = start;
     pdl_launch_dependents();
     const int page = 1 << p.page_log2, piece = min(page, DC_TILE), piece_log2 = min(p.page_log2, 6), pieces = DC_TILE >> piece_log2;
@@ -116,9 +127,8 @@ __global__ void __launch_bounds__(DC_THREADS, 2) paged_attn_decode_kernel(const 
         // ---- producer: lane i looks up the page of the item's piece `base + i`; K and V of a piece are issued by two lanes
         int s = 0, issued = 0;
         uint32_t parity = 1;                                                // a fresh barrier passes a wait on the previous phase
-        while (c.left > 0) {
+        for (int run; (run = c.run<DecodeRuns>()) > 0;) {
             int base = -64, ids = 0;
-            const int run = (int)min((long long)(c.s.n - c.at), c.left);
             for (int i = c.at; i < c.at + run && !failed; ++i) {
                 if ((i - base) * pieces >= 32 || base < 0) {                // the next 32 pieces' pages at once
                     base = i;
@@ -144,8 +154,7 @@ __global__ void __launch_bounds__(DC_THREADS, 2) paged_attn_decode_kernel(const 
                 if (++s == S::STAGES) s = 0, parity ^= 1u;
             }
             if (failed) break;
-            c.left -= run, c.at += run;
-            if (c.at == c.s.n) c.next(p, S::ROWS, DC_TILE);
+            c.advance<DecodeRuns>(p, S::ROWS, DC_TILE, run);
         }
         if (failed)                                                         // copies in flight end before the block does
             for (int k = 0; k < min(issued, S::STAGES); ++k) {
@@ -166,10 +175,10 @@ __global__ void __launch_bounds__(DC_THREADS, 2) paged_attn_decode_kernel(const 
         const uint32_t half_step = (uint32_t)piece * 128u;
         int s = 0;
         uint32_t parity = 0;
-        bool first_run = true;
+        int4 begun = make_int4(0, 0, 0, 0);
         int flags = 0;
-        while (c.left > 0) {
-            const int run = (int)min((long long)(c.s.n - c.at), c.left), from = c.at;
+        for (int run; (run = c.run<DecodeRuns>()) > 0;) {
+            const int from = c.at;
             uint32_t qf[NT][D / 16][2];
             int pos[NT][2];
 #pragma unroll
@@ -331,13 +340,11 @@ __global__ void __launch_bounds__(DC_THREADS, 2) paged_attn_decode_kernel(const 
                 for (int x = threadIdx.x; x < 2 * S::ROWS; x += 32 * DC_WARPS) part[S::ROWS * D + x] = sml[x];
                 flags |= from == 0 ? NOTE_BEGINS : NOTE_CONTINUES | (from + run == c.s.n ? NOTE_ENDS : 0);
             }
-            c.left -= run, c.at += run;
-            if (threadIdx.x == 0 && c.left == 0) p.notes[blockIdx.x] = make_int4(c.r, c.s.row0 / S::ROWS, c.h, flags);
-            if (c.at == c.s.n) c.next(p, S::ROWS, DC_TILE);
-            first_run = false;
+            if (!whole && from == 0) begun = make_int4(c.r, c.rb, c.h, 0);   // the last item of the run
+            c.advance<DecodeRuns>(p, S::ROWS, DC_TILE, run);
             consumer_barrier();                                              // the buffers are read
         }
-        if (first_run && threadIdx.x == 0) p.notes[blockIdx.x] = make_int4(0, 0, 0, 0);
+        if (threadIdx.x == 0) p.notes[blockIdx.x] = make_int4(begun.x, begun.y, begun.z, flags);
     }
     if (failed) atomicExch(p.status, KYB_DEV_TIMEOUT_ATTN);
 }

@@ -3,7 +3,8 @@
 // One persistent CTA an SM. A row block is two query tiles of 128 / G tokens (G query heads each: up to 128 rows, so the heads of a group share every key). Warps:
 //   0-3, 4-7   softmax of the first and the second query tile, one row a thread
 //   8          producer: query tiles, and a ring of 128-key tiles of K and V by tiled copies (one per page piece and half of the values)
-//   9          tcgen05.mma issuer (10 and 11 are idle: registers move between groups of four warps, from these four to the softmax)
+//   9          tcgen05.mma issuer
+//   10         clears values in places that no row sees (11 is idle: registers move between groups of four warps, from these four to the softmax)
 // Tensor memory: S0 | S1 | O0 | O1, 128 columns each; the weights P (16 bits) take the place of their scores S. S = Q K^T with both operands in shared memory; O += P V with
 // P in tensor memory and V as it lies in the cache (MN-major operand). The issuer's order S0(j+1) behind O0(j), S1(j+1) behind O1(j) keeps the tensor cores busy
 // with one query tile while the softmax of the other runs. A row's reference maximum moves only when a score passes it by 2^8, so O is rescaled (by the softmax warps
@@ -11,6 +12,7 @@
 // Keys that a row does not see are masked by selection in the tiles at the borders; values in places that no row of the block sees are cleared in shared memory, since such
 // places may hold anything and 0 times NaN is NaN.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged_attn.cuh"
 
@@ -18,11 +20,14 @@ namespace kyb {
 
 constexpr int PF_TILE = 128, PF_THREADS = 384;
 
+// An item costs about three tiles beyond its own (query load, the first scores, the last values, the output): measured.
+using PrefillRuns = Runs<3, 1>;
+
 template <int D>
 struct PrefillShape {
     static constexpr uint32_t HALVES = D / 64, HALF = 128 * 128, TILE = HALVES * HALF;       // a tile of 128 rows: halves of 64 values, 128-byte rows
-    static constexpr int SLOTS = D == 128 ? 5 : 10;
-    static constexpr uint32_t OFF_KV = 2 * TILE, OFF_BAR = OFF_KV + SLOTS * TILE, OFF_CUR = OFF_BAR + 16 * SLOTS + 64, SMEM = OFF_CUR + 8 * sizeof(Cursor);
+    static constexpr int SLOTS = 4 * 128 / D;                                // an even number: K in the even ones, V in the odd ones
+    static constexpr uint32_t OFF_KV = 2 * TILE, OFF_OUT = OFF_KV + SLOTS * TILE, OFF_BAR = OFF_OUT + 8 * 4096, OFF_CUR = OFF_BAR + 24 * SLOTS + 80, SMEM = OFF_CUR + 8 * sizeof(Cursor);
 };
 
 __device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&v)[16]) {
@@ -76,7 +81,7 @@ __device__ __forceinline__ int first_end_above(const int* v, int n, int x) {
 
 struct RunFinder {
     int tokens[PF_THREADS], kv[PF_THREADS], blocks_end[PF_THREADS];
-    unsigned long long tiles[PF_THREADS];
+    unsigned long long units[PF_THREADS];
     long long sums[PF_THREADS / 32];
     Cursor run;
     long long at;
@@ -99,7 +104,7 @@ __device__ __forceinline__ long long scan_block(long long v, long long* sums, lo
     }
     return v;
 }
-// tiles of up to PF_THREADS requests from r0 on, of all heads: the row blocks of all of them are shared among the threads
+// units of up to PF_THREADS requests from r0 on, of all heads: the row blocks of all of them are shared among the threads
 __device__ __forceinline__ long long count_chunk(const AttnParams& p, int block, int r0, RunFinder& f, long long& end) {
     const int tid = threadIdx.x, n = min(PF_THREADS, p.batch - r0);
     int nb = 0;
@@ -109,17 +114,22 @@ __device__ __forceinline__ long long count_chunk(const AttnParams& p, int block,
         f.tokens[tid] = request_rows(p, r0 + tid, base), f.kv[tid] = request_keys(p, r0 + tid);
         nb = row_blocks(p, f.tokens[tid], block);
     }
-    f.tiles[tid] = 0;
+    f.units[tid] = 0;
     long long all;
     f.blocks_end[tid] = (int)scan_block(nb, f.sums, all);
     __syncthreads();
-    for (int i = tid; i < (int)all; i += PF_THREADS) {
-        const int r = first_end_above(f.blocks_end, n, i), rb = i - (r ? f.blocks_end[r - 1] : 0);
-        atomicAdd(&f.tiles[r], (unsigned long long)key_span(p, f.tokens[r], f.kv[r], block, rb, PF_TILE).n * p.hkv);       // whole numbers: the order does not matter
+    for (int i0 = tid & ~31; i0 < (int)all; i0 += PF_THREADS) {              // whole numbers: the order of the additions does not matter
+        const int i = min(i0 + (tid & 31), (int)all - 1), r = first_end_above(f.blocks_end, n, i), rb = i - (r ? f.blocks_end[r - 1] : 0);
+        const int u = i0 + (tid & 31) < (int)all ? PrefillRuns::units(key_span(p, f.tokens[r], f.kv[r], block, rb, PF_TILE)) : 0;
+        const int r0_ = __shfl_sync(0xffffffffu, r, 0);
+        if (__all_sync(0xffffffffu, r == r0_)) {                             // one request's blocks, as usual: one addition for the warp
+            const int sum = __reduce_add_sync(0xffffffffu, u);
+            if ((tid & 31) == 0) atomicAdd(&f.units[r], (unsigned long long)sum * p.hkv);
+        } else if (u) atomicAdd(&f.units[r], (unsigned long long)u * p.hkv);
     }
     __syncthreads();
     long long total;
-    end = scan_block((long long)f.tiles[tid], f.sums, total);
+    end = scan_block((long long)f.units[tid], f.sums, total);
     return total;
 }
 // The run of tiles of CTA blockIdx.x, into f.run
@@ -129,13 +139,13 @@ __device__ __forceinline__ void find_run_wide(const AttnParams& p, int block, Ru
     for (int r0 = 0; r0 < p.batch; r0 += PF_THREADS) mine = count_chunk(p, block, r0, f, end), total += mine;
     const long long ctas = min((long long)gridDim.x, total), c = blockIdx.x;
     const long long u0 = c < ctas ? total * c / ctas : 0, u1 = c < ctas ? total * (c + 1) / ctas : 0;
-    if (tid == 0) f.run.left = u1 - u0;
+    if (tid == 0) f.run.left = 0;
     __syncthreads();
     if (u1 == u0) return;
     long long before = 0;
     for (int r0 = 0; r0 < p.batch && before <= u0; r0 += PF_THREADS) {
         if (p.batch > PF_THREADS) mine = count_chunk(p, block, r0, f, end);
-        const long long e = before + end, n = (long long)f.tiles[tid];
+        const long long e = before + end, n = (long long)f.units[tid];
         if (n && u0 >= e - n && u0 < e) f.request = r0 + tid, f.at = u0 - (e - n);
         before += mine;
         __syncthreads();
@@ -146,18 +156,43 @@ __device__ __forceinline__ void find_run_wide(const AttnParams& p, int block, Ru
     const int tokens = request_rows(p, r, base), kv = request_keys(p, r), nb = row_blocks(p, tokens, block);
     before = 0;
     for (int b0 = 0; b0 < nb && before <= at; b0 += PF_THREADS) {
-        const int rb = b0 + tid, one = rb < nb ? key_span(p, tokens, kv, block, rb, PF_TILE).n : 0;
+        const int rb = b0 + tid, one = rb < nb ? PrefillRuns::units(key_span(p, tokens, kv, block, rb, PF_TILE)) : 0;
         long long all;
         const long long e = before + scan_block((long long)one * p.hkv, f.sums, all), n = (long long)one * p.hkv;
         if (n && at >= e - n && at < e) {
             Cursor& k = f.run;
             k.r = r, k.rb = rb;
             k.load(p, block, PF_TILE);
-            k.h = (int)((at - (e - n)) / one), k.at = (int)((at - (e - n)) % one);
+            k.h = (int)((at - (e - n)) / one), k.left = u1 - u0;
+            k.at = PrefillRuns::enter(k.s, (int)((at - (e - n)) % one), k.left);
+            if (k.at == k.s.n) k.next(p, block, PF_TILE);
         }
         before += all;
         __syncthreads();
     }
+}
+
+// pairs of 32-bit values in one register pair
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ void split_pair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 
 template <typename T, int D>
@@ -166,13 +201,14 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_attn_prefill_kernel(const
     using S = PrefillShape<D>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u, kv0 = smem0 + S::OFF_KV;
-    const uint32_t full0 = smem0 + S::OFF_BAR, empty0 = full0 + 8 * S::SLOTS, qfull = empty0 + 8 * S::SLOTS, qempty = qfull + 8, sfull0 = qfull + 16, pfull0 = qfull + 32, tmem_slot = qfull + 48;
+    const uint32_t full0 = smem0 + S::OFF_BAR, empty0 = full0 + 8 * S::SLOTS, clean0 = empty0 + 8 * S::SLOTS, qfull = clean0 + 8 * S::SLOTS, qempty = qfull + 8, sfull0 = qfull + 16,
+                   pfull0 = qfull + 32, phalf0 = qfull + 48, tmem_slot = qfull + 64;      // pfull, phalf: the weights of a tile's first and second 64 keys
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int qrows = qtoks * p.group, block = 2 * qrows;                    // rows of a query tile, of a row block
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::SLOTS; ++s) mbar_init_a(full0 + 8 * s, 1), mbar_init_a(empty0 + 8 * s, 1);
+        for (int s = 0; s < S::SLOTS; ++s) mbar_init_a(full0 + 8 * s, 1), mbar_init_a(empty0 + 8 * s, 1), mbar_init_a(clean0 + 8 * s, 1);
         mbar_init_a(qfull, 1), mbar_init_a(qempty, 1);
-        for (int w = 0; w < 2; ++w) mbar_init_a(sfull0 + 8 * w, 1), mbar_init_a(pfull0 + 8 * w, 4);
+        for (int w = 0; w < 2; ++w) mbar_init_a(sfull0 + 8 * w, 1), mbar_init_a(pfull0 + 8 * w, 4), mbar_init_a(phalf0 + 8 * w, 4);
         mbar_fence_init();
         prefetch_tmap(&map_q), prefetch_tmap(&map_k), prefetch_tmap(&map_v);
     }
@@ -193,165 +229,188 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_attn_prefill_kernel(const
     // registers move from the producer's group of four warps to the softmax groups: 72 + 2 x 216 = 3 x 168, what the block was launched with
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-      if (warp == 8) {
-        // ---- producer: lane i looks up the page of the run's piece `base + i`; lanes issue the copies of a tile's pieces and halves
-        const int page = 1 << p.page_log2, piece = min(page, PF_TILE), piece_log2 = min(p.page_log2, 7), pieces = PF_TILE >> piece_log2, per_load = 32 / pieces;
         Cursor c = c0;
-        int s = 0, issued = 0;
-        uint32_t parity = 1, qparity = 1;
-        while (c.left > 0) {
-            const int run = (int)min((long long)(c.s.n - c.at), c.left);
-            const int tiles_q = c.s.rows > qrows ? 2 : 1;
-            if (!failed && !wait_here(qempty, qparity)) failed = true;
-            qparity ^= 1u;
-            if (!failed) {
-                if (lane == 0) mbar_expect_tx_a(qfull, (uint32_t)tiles_q * S::HALVES * (uint32_t)qrows * 128u);
-                __syncwarp();
-                if (lane < tiles_q * (int)S::HALVES) {
-                    const int w = lane / (int)S::HALVES, half = lane % (int)S::HALVES;
-                    tma_load_5d(smem0 + w * S::TILE + half * S::HALF, &map_q, 0, half, 0, c.h, c.row_base + c.s.row0 / p.group + w * qtoks, qfull);
-                }
-            }
-            auto lookup = [&](int i) {                                       // the pages of the pieces of tiles i, i + 1, ...
-                const int tl = i + lane / pieces, key = tl < c.s.n ? c.s.tile(tl) * PF_TILE + ((lane & (pieces - 1)) << piece_log2) : p.cap;
-                const bool seen = key < c.s.end && (key + piece > c.s.lo || key < p.sinks);
-                int id = seen ? p.table[c.r * p.ld_table + (key >> p.page_log2)] : p.pages;      // a piece that no row sees is read as if it lay behind the cache: zeros
-                return (unsigned)id >= (unsigned)p.pages ? p.pages : id;
-            };
-            int base = c.at, ids = lookup(base), ids_next = lookup(base + per_load);
-            for (int i = c.at; i < c.at + run && !failed; ++i) {
-                if (i - base == per_load) base = i, ids = ids_next, ids_next = lookup(base + per_load);
-                const int j = lane / (int)S::HALVES, half = lane % (int)S::HALVES;
-                const int id = __shfl_sync(0xffffffffu, ids, (i - base) * pieces + (j & (pieces - 1)));
-                const int y = (c.s.tile(i) * PF_TILE + (j << piece_log2)) & (page - 1);
-#pragma unroll
-                for (int kv = 0; kv < 2 && !failed; ++kv) {
-                    if (!wait_here(empty0 + 8 * s, parity)) {
-                        failed = true;
-                        break;
-                    }
-                    if (lane == 0) mbar_expect_tx_a(full0 + 8 * s, S::TILE);
-                    __syncwarp();
-                    if (j < pieces) tma_load_5d(kv0 + s * S::TILE + half * S::HALF + j * (piece * 128), kv ? &map_v : &map_k, 0, y, half, c.h, id, full0 + 8 * s);
-                    ++issued;
-                    if (++s == S::SLOTS) s = 0, parity ^= 1u;
-                }
-            }
-            c.left -= run, c.at += run;
-            if (c.at == c.s.n) c.next(p, block, PF_TILE);
-        }
-        if (failed)                                                          // copies in flight end before the block does
-            for (int k = 0; k < min(issued, S::SLOTS); ++k) {
-                const int at = issued - 1 - k;
-                wait_here(full0 + 8 * (at % S::SLOTS), (uint32_t)(at / S::SLOTS) & 1u);
-            }
-      } else if (warp == 9) {
-        // ---- issuer
-        Cursor c = c0;
-        constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
-        constexpr uint32_t idesc_s = umma_idesc_f16(128, 128) | fmt, idesc_o = umma_idesc_f16(128, D) | fmt | (1u << 16);      // V: MN-major
-        int s = 0;
-        uint32_t parity = 0, qparity = 0, pparity0 = 0, pparity1 = 0;
         auto wait = [&](uint32_t bar, uint32_t par) {
             if (!failed && !wait_here(bar, par)) failed = true;
-            tc_fence_after();
         };
-        auto scores = [&](int w, int slot) {                                 // S_w = Q_w K^T
+        if (warp == 8) {
+            // ---- producer: lane i looks up the page of the run's piece `base + i`; lanes issue the copies of a tile's pieces and halves
+            const int page = 1 << p.page_log2, piece = min(page, PF_TILE), piece_log2 = min(p.page_log2, 7), pieces = PF_TILE >> piece_log2, per_load = 32 / pieces;
+            const int j = lane / (int)S::HALVES, half = lane % (int)S::HALVES;
+            int s = 0, issued = 0;
+            uint32_t parity = 1, qparity = 1;                                // a fresh barrier passes a wait on the previous phase
+            for (int run; (run = c.run<PrefillRuns>()) > 0;) {
+                auto lookup = [&](int i) {                                   // the pages of the pieces of tiles i, i + 1, ...
+                    const int tl = i + lane / pieces, key = tl < c.s.n ? c.s.tile(tl) * PF_TILE + ((lane & (pieces - 1)) << piece_log2) : p.cap;
+                    const bool seen = key < c.s.end && (key + piece > c.s.lo || key < p.sinks);
+                    const int id = seen ? p.table[c.r * p.ld_table + (key >> p.page_log2)] : p.pages;      // a piece that no row sees is read as if it lay behind the cache: zeros
+                    return (unsigned)id >= (unsigned)p.pages ? p.pages : id;
+                };
+                int base = c.at, ids = lookup(base), ids_next = lookup(base + per_load);
+                for (int i = c.at; i < c.at + run; ++i) {
+                    if (i - base == per_load) base = i, ids = ids_next, ids_next = lookup(base + per_load);
+                    const int id = __shfl_sync(0xffffffffu, ids, (i - base) * pieces + (j & (pieces - 1)));
+                    const int y = (c.s.tile(i) * PF_TILE + (j << piece_log2)) & (page - 1);
 #pragma unroll
-            for (int h = 0; h < (int)S::HALVES; ++h) {
-                const uint64_t a = umma_desc_sw128(smem0 + w * S::TILE + h * S::HALF), b = umma_desc_sw128(kv0 + slot * S::TILE + h * S::HALF);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) umma_f16(tmem + 128 * w, a + 2 * k, b + 2 * k, idesc_s, (h | k) != 0);
-            }
-        };
-        auto values = [&](int w, int slot, bool first) {                     // O_w += P_w V
-            const uint64_t b = umma_desc_mn128(kv0 + slot * S::TILE, S::HALF);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) umma_f16_ts(tmem + 256 + 128 * w, tmem + 128 * w + 8 * k, b + 128 * k, idesc_o, !first || k);
-        };
-        while (c.left > 0) {
-            const int run = (int)min((long long)(c.s.n - c.at), c.left);
-            const bool two = c.s.rows > qrows;
-            wait(qfull, qparity);
-            qparity ^= 1u;
-            int slot_k = s;
-            wait(full0 + 8 * slot_k, parity);
-            if (++s == S::SLOTS) s = 0, parity ^= 1u;
-            if (!failed && elect_one()) {
-                scores(0, slot_k);
-                umma_commit(sfull0);
-                if (two) scores(1, slot_k), umma_commit(sfull0 + 8);
-                umma_commit(empty0 + 8 * slot_k);
-                if (run == 1) umma_commit(qempty);
-            }
-            __syncwarp();
-            for (int i = 0; i < run; ++i) {
-                const int slot_v = s;
-                wait(full0 + 8 * slot_v, parity);
-                if (++s == S::SLOTS) s = 0, parity ^= 1u;
-                const int key0 = c.s.tile(c.at + i) * PF_TILE;
-                if (!(key0 + PF_TILE <= c.s.end && (key0 >= c.s.lo || key0 + PF_TILE <= p.sinks)) && !failed) {
-                    // places that no row sees: their values become 0
-                    for (int x = lane; x < PF_TILE * (int)S::HALVES * 8; x += 32) {
-                        const int key = x / ((int)S::HALVES * 8), ch = x % ((int)S::HALVES * 8);
-                        if (!c.s.alive(key0 + key, p.sinks))
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(kv0 + slot_v * S::TILE + (ch >> 3) * S::HALF + key * 128 + (ch & 7) * 16), "r"(0) : "memory");
+                    for (int kv = 0; kv < 2; ++kv) {
+                        wait(empty0 + 8 * s, parity);
+                        if (!failed) {
+                            if (lane == 0) mbar_expect_tx_a(full0 + 8 * s, S::TILE);
+                            __syncwarp();
+                            if (j < pieces) tma_load_5d(kv0 + s * S::TILE + half * S::HALF + j * (piece * 128), kv ? &map_v : &map_k, 0, y, half, c.h, id, full0 + 8 * s);
+                            ++issued;
+                        }
+                        if (++s == S::SLOTS) s = 0, parity ^= 1u;
+                        if (kv == 0 && i == c.at) {                          // the queries, behind the first keys: their place is free only when the last scores are there
+                            const int tiles_q = c.s.rows > qrows ? 2 : 1;
+                            wait(qempty, qparity);
+                            qparity ^= 1u;
+                            if (!failed) {
+                                if (lane == 0) mbar_expect_tx_a(qfull, (uint32_t)tiles_q * S::HALVES * (uint32_t)qrows * 128u);
+                                __syncwarp();
+                                if (j < tiles_q) tma_load_5d(smem0 + j * S::TILE + half * S::HALF, &map_q, 0, half, 0, c.h, c.row_base + c.rb * 2 * qtoks + j * qtoks, qfull);
+                            }
+                        }
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
                 }
-                const bool more = i + 1 < run;
-                slot_k = s;
-                wait(pfull0, pparity0);
-                pparity0 ^= 1u;
-                if (!failed && elect_one()) values(0, slot_v, i == 0);
-                __syncwarp();
-                if (more) {
-                    wait(full0 + 8 * slot_k, parity);
-                    if (++s == S::SLOTS) s = 0, parity ^= 1u;
+                c.advance<PrefillRuns>(p, block, PF_TILE, run);
+            }
+            if (failed)                                                      // copies in flight end before the block does
+                for (int k = 0; k < min(issued, S::SLOTS); ++k) {
+                    const int at = issued - 1 - k;
+                    wait_here(full0 + 8 * (at % S::SLOTS), (uint32_t)(at / S::SLOTS) & 1u);
                 }
+        } else if (warp == 9) {
+            // ---- issuer
+            constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
+            constexpr uint32_t idesc_s = umma_idesc_f16(128, 128) | fmt, idesc_o = umma_idesc_f16(128, D) | fmt | (1u << 16);      // V: MN-major
+            int s = 0;
+            uint32_t parity = 0, qparity = 0, pparity0 = 0, pparity1 = 0;
+            auto next_slot = [&]() {
+                if (++s == S::SLOTS) s = 0, parity ^= 1u;
+            };
+            auto scores = [&](int w, int slot) {                             // S_w = Q_w K^T
+#pragma unroll
+                for (int h = 0; h < (int)S::HALVES; ++h) {
+                    const uint64_t a = umma_desc_sw128(smem0 + w * S::TILE + h * S::HALF), b = umma_desc_sw128(kv0 + slot * S::TILE + h * S::HALF);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) umma_f16(tmem + 128 * w, a + 2 * k, b + 2 * k, idesc_s, (h | k) != 0);
+                }
+            };
+            auto values = [&](int w, int slot, int half, bool first) {       // O_w += P_w V for 64 keys
+                const uint64_t b = umma_desc_mn128(kv0 + slot * S::TILE, S::HALF) + 512 * half;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) umma_f16_ts(tmem + 256 + 128 * w, tmem + 128 * w + 32 * half + 8 * k, b + 128 * k, idesc_o, !first || half || k);
+            };
+            for (int run; (run = c.run<PrefillRuns>()) > 0;) {
+                const bool two = c.s.rows > qrows;
+                int slot_k = s;
+                wait(full0 + 8 * slot_k, parity);
+                wait(qfull, qparity);
+                tc_fence_after();
+                qparity ^= 1u;
+                next_slot();
                 if (!failed && elect_one()) {
-                    if (more) scores(0, slot_k);
-                    umma_commit(sfull0);                                     // S0 of the next tile is there, O0 of this one too
+                    scores(0, slot_k);
+                    umma_commit(sfull0);
+                    if (two) scores(1, slot_k), umma_commit(sfull0 + 8);
+                    umma_commit(empty0 + 8 * slot_k);
+                    if (run == 1) umma_commit(qempty);
                 }
                 __syncwarp();
-                if (two) {
-                    wait(pfull0 + 8, pparity1);
-                    pparity1 ^= 1u;
+                for (int i = 0; i < run; ++i) {
+                    const int slot_v = s;
+                    wait(full0 + 8 * slot_v, parity);
+                    wait(clean0 + 8 * slot_v, parity);
+                    next_slot();
+                    const bool more = i + 1 < run;
+                    slot_k = s;
+                    wait(pfull0, pparity0);
+                    tc_fence_after();
+                    if (!failed && elect_one()) values(0, slot_v, 0, i == 0);
+                    __syncwarp();
+                    if (more) {
+                        wait(full0 + 8 * slot_k, parity);
+                        next_slot();
+                    }
+                    wait(phalf0, pparity0);
+                    tc_fence_after();
+                    pparity0 ^= 1u;
                     if (!failed && elect_one()) {
-                        values(1, slot_v, i == 0);
+                        values(0, slot_v, 1, i == 0);
+                        if (more) scores(0, slot_k);
+                        umma_commit(sfull0);                                 // S0 of the next tile is there, O0 of this one too
+                    }
+                    __syncwarp();
+                    if (two) {
+                        wait(pfull0 + 8, pparity1);
+                        tc_fence_after();
+                        if (!failed && elect_one()) values(1, slot_v, 0, i == 0);
+                        __syncwarp();
+                        wait(phalf0 + 8, pparity1);
+                        tc_fence_after();
+                        pparity1 ^= 1u;
+                        if (!failed && elect_one()) {
+                            values(1, slot_v, 1, i == 0);
+                            umma_commit(empty0 + 8 * slot_v);
+                            if (more) scores(1, slot_k);
+                            umma_commit(sfull0 + 8);
+                            if (more) umma_commit(empty0 + 8 * slot_k);
+                            if (i + 2 == run) umma_commit(qempty);
+                        }
+                    } else if (!failed && elect_one()) {
                         umma_commit(empty0 + 8 * slot_v);
-                        if (more) scores(1, slot_k);
-                        umma_commit(sfull0 + 8);
                         if (more) umma_commit(empty0 + 8 * slot_k);
                         if (i + 2 == run) umma_commit(qempty);
                     }
-                } else if (!failed && elect_one()) {
-                    umma_commit(empty0 + 8 * slot_v);
-                    if (more) umma_commit(empty0 + 8 * slot_k);
-                    if (i + 2 == run) umma_commit(qempty);
+                    __syncwarp();
                 }
-                __syncwarp();
+                c.advance<PrefillRuns>(p, block, PF_TILE, run);
             }
-            c.left -= run, c.at += run;
-            if (c.at == c.s.n) c.next(p, block, PF_TILE);
+        } else if (warp == 10) {
+            // ---- between producer and issuer: values in places that no row sees become 0 (the first and last tiles of an item)
+            int s = 1;
+            uint32_t parity = 0;
+            for (int run; (run = c.run<PrefillRuns>()) > 0;) {
+                for (int i = 0; i < run; ++i) {
+                    wait(full0 + 8 * s, parity);
+                    const int key0 = c.s.tile(c.at + i) * PF_TILE;
+                    // dead keys of the tile: [a0, a1) between the sinks and the window, [a2, 128) behind the last
+                    const int a1 = min(max(c.s.lo - key0, 0), PF_TILE), a0 = min(max(p.sinks - key0, 0), a1), a2 = max(min(c.s.end - key0, PF_TILE), 0);
+                    if ((a0 < a1 || a2 < PF_TILE) && !failed) {
+                        const uint32_t v = kv0 + s * S::TILE + (lane >> 3 & (S::HALVES - 1)) * S::HALF + (lane & 7) * 16;
+                        for (int k = a0 + lane / (8 * (int)S::HALVES); k < PF_TILE; k += 32 / (8 * (int)S::HALVES)) {
+                            if (k >= a1 && k < a2) continue;
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v + k * 128), "r"(0) : "memory");
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                    }
+                    if (lane == 0) mbar_arrive_a(clean0 + 8 * s);
+                    s += 2;
+                    if (s > S::SLOTS) s = 1, parity ^= 1u;
+                }
+                c.advance<PrefillRuns>(p, block, PF_TILE, run);
+            }
         }
-      }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         // ---- softmax: one row a thread
         const int w = warp >> 2, rl = (warp & 3) * 32 + lane;
-        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lane_base + 128u * w, to = ts + 256u, sfull = sfull0 + 8 * w, pfull = pfull0 + 8 * w;
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lane_base + 128u * w, to = ts + 256u, sfull = sfull0 + 8 * w, pfull = pfull0 + 8 * w, phalf = phalf0 + 8 * w;
+        const uint32_t stage = smem0 + S::OFF_OUT + warp * 4096;             // 32 rows x 128 bytes on their way to memory
         const float scale2 = fabsf(p.scale2);
+        const uint64_t scale_pair = pair_of(scale2, scale2);
         const bool flip = p.scale2 < 0.f;
         uint32_t sparity = 0;
         int flags = 0;
         // the warp's place in its run lies in shared memory: a row's 128 scores take the registers
         Cursor& c = *reinterpret_cast<Cursor*>(smem_raw + (smem0 - smem_u32(smem_raw)) + S::OFF_CUR + warp * sizeof(Cursor));
         if (lane == 0) c = c0;
+        if (threadIdx.x == 0) p.notes[blockIdx.x] = make_int4(0, 0, 0, 0);
         __syncwarp();
-        while (c.left > 0) {
-            const int from = c.at, run = (int)min((long long)(c.s.n - from), c.left);
+        for (int run; (run = c.run<PrefillRuns>()) > 0;) {
+            const int from = c.at;
             const int row = w * qrows + rl;                                  // row of the block
             const bool on = rl < qrows && row < c.s.rows;
             float m = -INFINITY, l = 0.f;
@@ -364,8 +423,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_attn_prefill_kernel(const
                     sparity ^= 1u;
                     tc_fence_after();
                     uint32_t v[4][32];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) tmem_ld_32x32(ts + 32 * q, v[q]);
+                    tmem_ld_32x32(ts, v[0]);
+                    tmem_ld_32x32(ts + 32, v[1]);
+                    tmem_ld_32x32(ts + 64, v[2]);
+                    tmem_ld_32x32(ts + 96, v[3]);
                     tmem_ld_wait();
                     const int key0 = (from + i + (from + i < sink_tiles ? 0 : main_tile)) * PF_TILE;
                     if (flip)
@@ -374,24 +435,26 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_attn_prefill_kernel(const
 #pragma unroll
                             for (int e = 0; e < 32; ++e) v[q][e] ^= 0x80000000u;
                     if (key0 > plain_hi || key0 < plain_lo) {
-                        const int hi = min(pos, p.cap - 1) - key0, lo = p.window ? pos - p.window + 1 - key0 : -1, sk = p.sinks - key0;
+                        // keys up to hi, from lo on or below sk are seen: 32 of them a mask word
+                        const int hi = min(pos, p.cap - 1) - key0, lo = p.window ? pos - p.window + 1 - key0 : 0, sk = p.sinks - key0;
+                        auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
 #pragma unroll
-                        for (int q = 0; q < 4; ++q)
+                        for (int q = 0; q < 4; ++q) {
+                            const uint32_t see = below(hi + 1 - 32 * q) & (~below(lo - 32 * q) | below(sk - 32 * q));
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                const int col = 32 * q + e;
-                                if (!(col <= hi && (col >= lo || col < sk))) v[q][e] = 0xff800000u;
-                            }
+                            for (int e = 0; e < 32; ++e)
+                                if (!(see >> e & 1u)) v[q][e] = 0xff800000u;
+                        }
                     }
                     float t[4];
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        float a = __uint_as_float(v[q][0]);
+                        float a = max3(__uint_as_float(v[q][0]), __uint_as_float(v[q][1]), __uint_as_float(v[q][2]));
 #pragma unroll
-                        for (int e = 1; e < 32; ++e) a = fmaxf(a, __uint_as_float(v[q][e]));
-                        t[q] = a;
+                        for (int e = 3; e < 31; e += 2) a = max3(a, __uint_as_float(v[q][e]), __uint_as_float(v[q][e + 1]));
+                        t[q] = fmaxf(a, __uint_as_float(v[q][31]));
                     }
-                    const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * scale2;
+                    const float top = fmaxf(max3(t[0], t[1], t[2]), t[3]) * scale2;
                     const bool over = top > m + 8.f;                         // false where nothing is seen yet (-inf on both sides)
                     if (__any_sync(0xffffffffu, over)) {
                         const float f = !over ? 1.f : m == -INFINITY ? 0.f : exp2_fast(m - top);
@@ -409,69 +472,94 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_attn_prefill_kernel(const
                             }
                         }
                     }
-                    const float m0 = m == -INFINITY ? 0.f : m;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    const float m0 = m == -INFINITY ? 0.f : -m;
+                    const uint64_t m_pair = pair_of(m0, m0);
+                    uint64_t sum0 = 0, sum1 = 0;                             // two pairs of zeros
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         uint32_t pk[16];
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) {
-                            const float a = exp2_fast(fmaf(__uint_as_float(v[q][e]), scale2, -m0)), b = exp2_fast(fmaf(__uint_as_float(v[q][e + 1]), scale2, -m0));
-                            sum[(e >> 1) & 3] += a + b;
+                            float a, b;
+                            split_pair(fma_pair(pair_of(__uint_as_float(v[q][e]), __uint_as_float(v[q][e + 1])), scale_pair, m_pair), a, b);
+                            a = exp2_fast(a), b = exp2_fast(b);
+                            if (e & 2) sum1 = add_pair(sum1, pair_of(a, b)); else sum0 = add_pair(sum0, pair_of(a, b));
                             pk[e / 2] = pack2<T>(a, b);
                         }
                         tmem_st_16(ts + 16 * q, pk);
+                        if (q & 1) {                                         // the weights of 64 keys are there
+                            tmem_st_wait_all();
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive_a(q == 1 ? pfull : phalf);
+                        }
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    tmem_st_wait_all();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_a(pfull);
+                    float a, b;
+                    split_pair(add_pair(sum0, sum1), a, b);
+                    l += a + b;
                 }
                 if (!failed && !wait_here(sfull, sparity)) failed = true;    // the last O
                 sparity ^= 1u;
                 tc_fence_after();
-                const float inv = l > 0.f ? 1.f / l : 0.f;
+                // ---- output: 128 bytes of each of the warp's rows at a time through shared memory (16-byte pieces, swizzled), so that eight lanes store one row's
                 const bool whole = from == 0 && run == c.s.n;
+                const float inv = !whole ? 1.f : l > 0.f ? 1.f / l : 0.f;
                 const int tok = (c.s.row0 + row) / p.group;
-                T* const out = reinterpret_cast<T*>(p.o) + (int64_t)(c.row_base + (on ? tok : 0)) * p.o_t + (int64_t)(c.h * p.group + (on ? c.s.row0 + row - tok * p.group : 0)) * p.o_h;
-                float* const part = p.parts + ((size_t)blockIdx.x * 2 + (from == 0)) * ((size_t)block * (D + 2)) + (size_t)row * D;
+                const uint32_t row_bytes = whole ? D * 2 : D * 4;
+                uint8_t* mine = whole ? p.o + 2 * ((int64_t)(c.row_base + tok) * p.o_t + (int64_t)(c.h * p.group + c.s.row0 + row - tok * p.group) * p.o_h)
+                                      : reinterpret_cast<uint8_t*>(p.parts + ((size_t)blockIdx.x * 2 + (from == 0)) * ((size_t)block * (D + 2)) + (size_t)row * D);
+                if (on && !whole && !failed) {
+                    float* const ml = p.parts + ((size_t)blockIdx.x * 2 + (from == 0)) * ((size_t)block * (D + 2)) + (size_t)block * D + row;
+                    ml[0] = m, ml[block] = l;
+                }
+                if (!on || failed) mine = nullptr;
 #pragma unroll 1
-                for (int q = 0; q < D; q += 32) {
-                    uint32_t x[32];
-                    tmem_ld_32x32(to + q, x);
-                    tmem_ld_wait();
-                    if (!on || failed) continue;
+                for (uint32_t off = 0; off < row_bytes; off += 128) {
+                    __syncwarp();
                     if (whole) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            uint4 y;
-                            y.x = pack2<T>(__uint_as_float(x[e]) * inv, __uint_as_float(x[e + 1]) * inv), y.y = pack2<T>(__uint_as_float(x[e + 2]) * inv, __uint_as_float(x[e + 3]) * inv);
-                            y.z = pack2<T>(__uint_as_float(x[e + 4]) * inv, __uint_as_float(x[e + 5]) * inv), y.w = pack2<T>(__uint_as_float(x[e + 6]) * inv, __uint_as_float(x[e + 7]) * inv);
-                            *reinterpret_cast<uint4*>(out + q + e) = y;
+                        for (int h = 0; h < 2; ++h) {
+                            uint32_t x[32];
+                            tmem_ld_32x32(to + off / 2 + 32 * h, x);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                uint32_t y[4];
+#pragma unroll
+                                for (int u = 0; u < 4; ++u) y[u] = pack2<T>(__uint_as_float(x[8 * e + 2 * u]) * inv, __uint_as_float(x[8 * e + 2 * u + 1]) * inv);
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 + (((4 * h + e) ^ (lane & 7)) << 4)), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
+                            }
                         }
                     } else {
+                        uint32_t x[32];
+                        tmem_ld_32x32(to + off / 4, x);
+                        tmem_ld_wait();
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            *reinterpret_cast<float4*>(part + q + e) = make_float4(__uint_as_float(x[e]), __uint_as_float(x[e + 1]), __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+                        for (int e = 0; e < 8; ++e)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 + ((e ^ (lane & 7)) << 4)), "r"(x[4 * e]), "r"(x[4 * e + 1]), "r"(x[4 * e + 2]), "r"(x[4 * e + 3])
+                                         : "memory");
                     }
-                }
-                if (on && !whole && !failed) {
-                    float* const ml = part - (size_t)row * D + (size_t)block * D + row;
-                    ml[0] = m, ml[block] = l;
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int r = 4 * k + (lane >> 3);
+                        uint8_t* const to_row = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), r));
+                        const uint4 y = lds128(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+                        if (to_row) *reinterpret_cast<uint4*>(to_row + off + (lane & 7) * 16) = y;
+                    }
                 }
                 tc_fence_before();
             }
             __syncwarp();
             if (lane == 0) {
-                if (from != 0 || run != c.s.n) flags |= from == 0 ? NOTE_BEGINS : NOTE_CONTINUES | (from + run == c.s.n ? NOTE_ENDS : 0);
-                c.left -= run, c.at += run;
-                if (warp == 0 && c.left == 0) p.notes[blockIdx.x] = make_int4(c.r, c.s.row0 / block, c.h, flags);
-                if (c.at == c.s.n) c.next(p, block, PF_TILE);
+                if (from != 0 || run != c.s.n) {
+                    flags |= from == 0 ? NOTE_BEGINS : NOTE_CONTINUES | (from + run == c.s.n ? NOTE_ENDS : 0);
+                    if (warp == 0) p.notes[blockIdx.x] = make_int4(c.r, c.rb, c.h, flags);
+                }
+                c.advance<PrefillRuns>(p, block, PF_TILE, run);
             }
             __syncwarp();
         }
-        if (c0.left == 0 && threadIdx.x == 0) p.notes[blockIdx.x] = make_int4(0, 0, 0, 0);
     }
     if (failed) atomicExch(p.status, KYB_DEV_TIMEOUT_ATTN);
     tc_fence_before();
@@ -518,6 +606,7 @@ int launch_prefill(KybAttnCall& c, void* ws) {
     if (int rc = make_query_map(&mq, c, qtoks)) return rc;
     if (int rc = kyb_make_cache_map(&mk, c.k, c.dtype, c.p.pages, c.p.hkv, c.page, D, c.k_p, c.k_h, piece, 1)) return rc;
     if (int rc = kyb_make_cache_map(&mv, c.v, c.dtype, c.p.pages, c.p.hkv, c.page, D, c.v_p, c.v_h, piece, 1)) return rc;
+    c.p.block_tokens = 2 * qtoks;
     c.p.notes = (int4*)ws, c.p.parts = (float*)((char*)ws + (size_t)ctas * sizeof(int4));
     kern<<<(unsigned)ctas, kyb::PF_THREADS, S::SMEM + 1024, c.st>>>(mq, mk, mv, c.p, qtoks);
     if (int rc = kyb_launch_check("paged_attn_prefill")) return rc;
