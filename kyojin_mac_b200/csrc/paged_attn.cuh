@@ -72,7 +72,7 @@ template <int OVER, int SNAP>
 struct Runs {
     static __device__ __forceinline__ int units(const KeySpan& s) { return s.n + OVER; }
     // a run that starts `x` units into an item: the tile it starts with (n: with the next item), and what changes in its number of units
-    static __device__ __forceinline__ int enter(const KeySpan& s, int x, long long& left) {
+    static __device__ __forceinline__ int enter(const KeySpan& s, int x, int& left) {
         if (x > OVER && s.n + OVER - x <= SNAP) {
             left -= s.n + OVER - x;
             return s.n;
@@ -84,17 +84,23 @@ struct Runs {
         return x - OVER;
     }
     // tiles of the item that a run with `left` units takes from tile `at` on (0: the run ends in front of it)
-    static __device__ __forceinline__ int take(const KeySpan& s, int at, long long left) {
-        const long long n = left - (at ? 0 : OVER);
-        return n <= 0 ? 0 : n + SNAP >= s.n - at ? s.n - at : (int)n;
+    static __device__ __forceinline__ int take(const KeySpan& s, int at, int left) {
+        const int n = left - (at ? 0 : OVER);
+        return n <= 0 ? 0 : n + SNAP >= s.n - at ? s.n - at : n;
     }
     static __device__ __forceinline__ int cost(int at, int taken) { return taken + (at ? 0 : OVER); }
 };
 
+// border c of `runs` equal runs over `total` units (fewer than 2^31, the host sees to it)
+__device__ __forceinline__ int run_border(int total, int runs, int c) {
+    const int each = total / runs;
+    return each * c + min(c, total - each * runs);
+}
+
 // Where a CTA's run is
 struct Cursor {
     int r, rb, h, at;          // request, row block, head, next tile of the item
-    long long left;            // units left in the run
+    int left;                  // units left in the run
     int tokens, kv, blocks, row_base;
     KeySpan s;
     __device__ __forceinline__ void load(const AttnParams& p, int block, int tile) {
@@ -186,6 +192,11 @@ struct KybAttnCall {
     int d, dtype, page, sms;
     cudaStream_t st;
 };
+// an upper bound of the units that the kernels deal out: row blocks (each request's last may be a part) x heads x tiles of a full table row and an item's extra
+static inline bool kyb_attn_units_fit(const KybAttnCall& c, int block, int tile) {
+    const int64_t blocks = c.tokens * c.p.group / block + c.p.batch, tiles = (int64_t)c.p.cap / tile + 8;
+    return blocks * c.p.hkv < (1ll << 31) / tiles;
+}
 // rows a request may bring for the decode kernel; beyond, the prefill kernel
 constexpr int KYB_DECODE_ROWS = 16;
 size_t kyb_attn_decode_scratch(int d, int rows, int sms);

@@ -42,43 +42,42 @@ struct DecodeShape {
 };
 
 using DecodeRuns = Runs<1, 0>;
-__device__ __forceinline__ long long request_units(const AttnParams& p, int r, int block) {
+__device__ __forceinline__ int request_units(const AttnParams& p, int r, int block) {
     int base;
     const int tokens = request_rows(p, r, base), kv = request_keys(p, r), nb = row_blocks(p, tokens, block);
-    long long n = 0;
+    int n = 0;
     for (int b = 0; b < nb; ++b) n += DecodeRuns::units(key_span(p, tokens, kv, block, b, DC_TILE));
     return n * p.hkv;
 }
 
 // First item and length of this CTA's run: every thread of the block takes part; the result is in *out (shared).
-__device__ __forceinline__ void find_run(const AttnParams& p, int block, Cursor* out, long long* sums, int threads) {
+__device__ __forceinline__ void find_run(const AttnParams& p, int block, Cursor* out, int* sums, int threads) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = threads / 32;
-    long long mine = 0;
+    int mine = 0;
     for (int r = tid; r < p.batch; r += threads) mine += request_units(p, r, block);
-    const long long first = mine;                                           // (this thread's only request when there are no more of them than threads)
-#pragma unroll
-    for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+    const int first = mine;                                                 // (this thread's only request when there are no more of them than threads)
+    mine = __reduce_add_sync(0xffffffffu, mine);
     if (lane == 0) sums[warp] = mine;
     if (tid == 0) out->left = 0;
     __syncthreads();
-    long long total = 0;
+    int total = 0;
     for (int w = 0; w < warps; ++w) total += sums[w];
-    const long long ctas = min((long long)gridDim.x, total), c = blockIdx.x;
-    const long long u0 = c < ctas ? total * c / ctas : 0, u1 = c < ctas ? total * (c + 1) / ctas : 0;
+    const int ctas = min((int)gridDim.x, total), c = blockIdx.x;
+    const int u0 = c < ctas ? run_border(total, ctas, c) : 0, u1 = c < ctas ? run_border(total, ctas, c + 1) : 0;
     __syncthreads();
-    long long before = 0;
+    int before = 0;
     for (int r0 = 0; r0 < p.batch && u1 > u0 && before <= u0; r0 += threads) {
         const int r = r0 + tid;
-        const long long n = r < p.batch ? (p.batch <= threads ? first : request_units(p, r, block)) : 0;
-        long long end = n;
+        const int n = r < p.batch ? (p.batch <= threads ? first : request_units(p, r, block)) : 0;
+        int end = n;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, end, d);
+            const int x = __shfl_up_sync(0xffffffffu, end, d);
             if (lane >= d) end += x;
         }
         if (lane == 31) sums[warp] = end;
         __syncthreads();
-        long long all = before;
+        int all = before;
         for (int w = 0; w < warps; ++w) {
             if (w < warp) end += sums[w];
             all += sums[w];
@@ -86,12 +85,12 @@ __device__ __forceinline__ void find_run(const AttnParams& p, int block, Cursor*
         end += before;
         if (u0 >= end - n && u0 < end) {
             Cursor k;
-            long long at = u0 - (end - n);
+            int at = u0 - (end - n);
             k.r = r, k.rb = 0, k.left = u1 - u0;
             k.load(p, block, DC_TILE);
-            while (at >= (long long)DecodeRuns::units(k.s) * p.hkv) at -= (long long)DecodeRuns::units(k.s) * p.hkv, ++k.rb, k.s = key_span(p, k.tokens, k.kv, block, k.rb, DC_TILE);
-            k.h = (int)(at / DecodeRuns::units(k.s));
-            k.at = DecodeRuns::enter(k.s, (int)(at % DecodeRuns::units(k.s)), k.left);
+            while (at >= DecodeRuns::units(k.s) * p.hkv) at -= DecodeRuns::units(k.s) * p.hkv, ++k.rb, k.s = key_span(p, k.tokens, k.kv, block, k.rb, DC_TILE);
+            k.h = at / DecodeRuns::units(k.s);
+            k.at = DecodeRuns::enter(k.s, at - k.h * DecodeRuns::units(k.s), k.left);
             if (k.at == k.s.n) k.next(p, block, DC_TILE);
             *out = k;
         }
@@ -106,7 +105,7 @@ __global__ void __launch_bounds__(DC_THREADS, 2) paged_attn_decode_kernel(const 
     using S = DecodeShape<D, NT>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ Cursor start;
-    __shared__ long long sums[DC_WARPS + 1];
+    __shared__ int sums[DC_WARPS + 1];
     const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* const smem_g = smem_raw + (smem0 - smem_u32(smem_raw));
     const uint32_t full0 = smem0 + S::OFF_BAR, empty0 = full0 + 8 * S::STAGES;
@@ -417,6 +416,7 @@ int launch_decode(KybAttnCall& c, void* ws) {
     using S = kyb::DecodeShape<D, NT>;
     auto kern = kyb::paged_attn_decode_kernel<T, D, NT>;
     if (int rc = kyb_allow_smem((const void*)kern)) return rc;
+    KYB_REQUIRE(kyb_attn_units_fit(c, S::ROWS, kyb::DC_TILE), "more than 2^31 key tiles in one call: split it");
     const int ctas = DC_PER_SM * c.sms, piece = std::min(c.page, kyb::DC_TILE);
     CUtensorMap mk, mv;
     if (int rc = kyb_make_cache_map(&mk, c.k, c.dtype, c.p.pages, c.p.hkv, c.page, D, c.k_p, c.k_h, piece, D / 64)) return rc;

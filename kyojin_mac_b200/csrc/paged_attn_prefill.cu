@@ -80,24 +80,22 @@ __device__ __forceinline__ int first_end_above(const int* v, int n, int x) {
 }
 
 struct RunFinder {
-    int tokens[PF_THREADS], kv[PF_THREADS], blocks_end[PF_THREADS];
-    unsigned long long units[PF_THREADS];
-    long long sums[PF_THREADS / 32];
+    int tokens[PF_THREADS], kv[PF_THREADS], blocks_end[PF_THREADS], units[PF_THREADS], sums[2][PF_THREADS / 32];
     Cursor run;
-    long long at;
-    int request;
+    int at, request;
 };
-__device__ __forceinline__ long long scan_block(long long v, long long* sums, long long& total) {
+// inclusive sum over the block; two calls in a row use two places for the warps' sums, so that one barrier a call is enough
+__device__ __forceinline__ int scan_block(int v, int* sums, int& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, v, d);
+        const int x = __shfl_up_sync(0xffffffffu, v, d);
         if (lane >= d) v += x;
     }
-    __syncthreads();
     if (lane == 31) sums[warp] = v;
     __syncthreads();
     total = 0;
+#pragma unroll
     for (int w = 0; w < PF_THREADS / 32; ++w) {
         if (w < warp) v += sums[w];
         total += sums[w];
@@ -105,70 +103,73 @@ __device__ __forceinline__ long long scan_block(long long v, long long* sums, lo
     return v;
 }
 // units of up to PF_THREADS requests from r0 on, of all heads: the row blocks of all of them are shared among the threads
-__device__ __forceinline__ long long count_chunk(const AttnParams& p, int block, int r0, RunFinder& f, long long& end) {
+__device__ __forceinline__ int count_chunk(const AttnParams& p, int block, int r0, RunFinder& f, int& end) {
     const int tid = threadIdx.x, n = min(PF_THREADS, p.batch - r0);
     int nb = 0;
-    __syncthreads();
     if (tid < n) {
         int base;
         f.tokens[tid] = request_rows(p, r0 + tid, base), f.kv[tid] = request_keys(p, r0 + tid);
         nb = row_blocks(p, f.tokens[tid], block);
     }
     f.units[tid] = 0;
-    long long all;
-    f.blocks_end[tid] = (int)scan_block(nb, f.sums, all);
+    int all;
+    f.blocks_end[tid] = scan_block(nb, f.sums[0], all);
     __syncthreads();
-    for (int i0 = tid & ~31; i0 < (int)all; i0 += PF_THREADS) {              // whole numbers: the order of the additions does not matter
-        const int i = min(i0 + (tid & 31), (int)all - 1), r = first_end_above(f.blocks_end, n, i), rb = i - (r ? f.blocks_end[r - 1] : 0);
-        const int u = i0 + (tid & 31) < (int)all ? PrefillRuns::units(key_span(p, f.tokens[r], f.kv[r], block, rb, PF_TILE)) : 0;
-        const int r0_ = __shfl_sync(0xffffffffu, r, 0);
-        if (__all_sync(0xffffffffu, r == r0_)) {                             // one request's blocks, as usual: one addition for the warp
+    for (int i0 = tid & ~31; i0 < all; i0 += PF_THREADS) {                   // whole numbers: the order of the additions does not matter
+        const int i = min(i0 + (tid & 31), all - 1), r = first_end_above(f.blocks_end, n, i), rb = i - (r ? f.blocks_end[r - 1] : 0);
+        const int u = i0 + (tid & 31) < all ? PrefillRuns::units(key_span(p, f.tokens[r], f.kv[r], block, rb, PF_TILE)) * p.hkv : 0;
+        const int r_first = __shfl_sync(0xffffffffu, r, 0);
+        if (__all_sync(0xffffffffu, r == r_first)) {                         // one request's blocks, as usual: one addition for the warp
             const int sum = __reduce_add_sync(0xffffffffu, u);
-            if ((tid & 31) == 0) atomicAdd(&f.units[r], (unsigned long long)sum * p.hkv);
-        } else if (u) atomicAdd(&f.units[r], (unsigned long long)u * p.hkv);
+            if ((tid & 31) == 0) atomicAdd(&f.units[r], sum);
+        } else if (u) atomicAdd(&f.units[r], u);
     }
     __syncthreads();
-    long long total;
-    end = scan_block((long long)f.units[tid], f.sums, total);
+    int total;
+    end = scan_block(f.units[tid], f.sums[1], total);
     return total;
 }
 // The run of tiles of CTA blockIdx.x, into f.run
 __device__ __forceinline__ void find_run_wide(const AttnParams& p, int block, RunFinder& f) {
     const int tid = threadIdx.x;
-    long long total = 0, end = 0, mine = 0;
-    for (int r0 = 0; r0 < p.batch; r0 += PF_THREADS) mine = count_chunk(p, block, r0, f, end), total += mine;
-    const long long ctas = min((long long)gridDim.x, total), c = blockIdx.x;
-    const long long u0 = c < ctas ? total * c / ctas : 0, u1 = c < ctas ? total * (c + 1) / ctas : 0;
+    int total = 0, end = 0, mine = 0;
+    for (int r0 = 0; r0 < p.batch; r0 += PF_THREADS) {
+        if (r0) __syncthreads();
+        mine = count_chunk(p, block, r0, f, end), total += mine;
+    }
+    const int ctas = min((int)gridDim.x, total), c = blockIdx.x;
+    const int u0 = c < ctas ? run_border(total, ctas, c) : 0, u1 = c < ctas ? run_border(total, ctas, c + 1) : 0;
     if (tid == 0) f.run.left = 0;
-    __syncthreads();
     if (u1 == u0) return;
-    long long before = 0;
+    int before = 0;
     for (int r0 = 0; r0 < p.batch && before <= u0; r0 += PF_THREADS) {
-        if (p.batch > PF_THREADS) mine = count_chunk(p, block, r0, f, end);
-        const long long e = before + end, n = (long long)f.units[tid];
+        if (p.batch > PF_THREADS) {
+            __syncthreads();
+            mine = count_chunk(p, block, r0, f, end);
+        }
+        const int e = before + end, n = f.units[tid];
         if (n && u0 >= e - n && u0 < e) f.request = r0 + tid, f.at = u0 - (e - n);
         before += mine;
-        __syncthreads();
     }
-    const int r = f.request;
-    const long long at = f.at;
+    __syncthreads();
+    const int r = f.request, at = f.at;
     int base;
     const int tokens = request_rows(p, r, base), kv = request_keys(p, r), nb = row_blocks(p, tokens, block);
     before = 0;
     for (int b0 = 0; b0 < nb && before <= at; b0 += PF_THREADS) {
-        const int rb = b0 + tid, one = rb < nb ? PrefillRuns::units(key_span(p, tokens, kv, block, rb, PF_TILE)) : 0;
-        long long all;
-        const long long e = before + scan_block((long long)one * p.hkv, f.sums, all), n = (long long)one * p.hkv;
+        const int rb = b0 + tid, one = rb < nb ? PrefillRuns::units(key_span(p, tokens, kv, block, rb, PF_TILE)) : 0, n = one * p.hkv;
+        int all;
+        const int e = before + scan_block(n, f.sums[b0 / PF_THREADS & 1], all);
         if (n && at >= e - n && at < e) {
             Cursor& k = f.run;
-            k.r = r, k.rb = rb;
+            const int x = at - (e - n);
+            k.r = r, k.rb = rb, k.left = u1 - u0;
             k.load(p, block, PF_TILE);
-            k.h = (int)((at - (e - n)) / one), k.left = u1 - u0;
-            k.at = PrefillRuns::enter(k.s, (int)((at - (e - n)) % one), k.left);
+            k.h = x / one;
+            k.at = PrefillRuns::enter(k.s, x - k.h * one, k.left);
             if (k.at == k.s.n) k.next(p, block, PF_TILE);
         }
         before += all;
-        __syncthreads();
     }
 }
 
@@ -281,92 +282,86 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_attn_prefill_kernel(const
                     wait_here(full0 + 8 * (at % S::SLOTS), (uint32_t)(at / S::SLOTS) & 1u);
                 }
         } else if (warp == 9) {
-            // ---- issuer
+            // ---- issuer. The whole warp runs this, its conditions are votes and reductions and one elected lane issues, so that addresses and descriptors stay in uniform
+            // registers: with operands in vector registers an MMA took 75 clocks to issue, more than it runs.
             constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
             constexpr uint32_t idesc_s = umma_idesc_f16(128, 128) | fmt, idesc_o = umma_idesc_f16(128, D) | fmt | (1u << 16);      // V: MN-major
-            int s = 0;
-            uint32_t parity = 0, qparity = 0, pparity0 = 0, pparity1 = 0;
-            auto next_slot = [&]() {
-                if (++s == S::SLOTS) s = 0, parity ^= 1u;
-            };
-            auto scores = [&](int w, int slot) {                             // S_w = Q_w K^T
+            const bool lead = elect_one();
+            const uint32_t td = __reduce_max_sync(0xffffffffu, tmem);
+            const uint64_t desc_q = umma_desc_sw128(smem0), desc_k = umma_desc_sw128(kv0), desc_v = umma_desc_mn128(kv0, S::HALF);
+            uint32_t n = 0, items = 0, p0 = 0, p1 = 0;                       // slots, items and weights of either query tile so far
+            bool ok = true;
+            auto scores = [&](uint32_t w, uint32_t slot) {                   // S_w = Q_w K^T
 #pragma unroll
-                for (int h = 0; h < (int)S::HALVES; ++h) {
-                    const uint64_t a = umma_desc_sw128(smem0 + w * S::TILE + h * S::HALF), b = umma_desc_sw128(kv0 + slot * S::TILE + h * S::HALF);
+                for (uint32_t h = 0; h < S::HALVES; ++h)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) umma_f16(tmem + 128 * w, a + 2 * k, b + 2 * k, idesc_s, (h | k) != 0);
-                }
+                    for (uint32_t k = 0; k < 4; ++k)
+                        umma_f16(td + 128 * w, desc_q + (w * S::TILE + h * S::HALF) / 16 + 2 * k, desc_k + slot * (S::TILE / 16) + h * (S::HALF / 16) + 2 * k, idesc_s, (h | k) != 0);
             };
-            auto values = [&](int w, int slot, int half, bool first) {       // O_w += P_w V for 64 keys
-                const uint64_t b = umma_desc_mn128(kv0 + slot * S::TILE, S::HALF) + 512 * half;
+            auto values = [&](uint32_t w, uint32_t slot, uint32_t half, uint32_t acc) {       // O_w += P_w V for 64 keys
 #pragma unroll
-                for (int k = 0; k < 4; ++k) umma_f16_ts(tmem + 256 + 128 * w, tmem + 128 * w + 32 * half + 8 * k, b + 128 * k, idesc_o, !first || half || k);
+                for (uint32_t k = 0; k < 4; ++k)
+                    umma_f16_ts(td + 256 + 128 * w, td + 128 * w + 32 * half + 8 * k, desc_v + slot * (S::TILE / 16) + 512 * half + 128 * k, idesc_o, half || k ? 1u : acc);
             };
-            for (int run; (run = c.run<PrefillRuns>()) > 0;) {
-                const bool two = c.s.rows > qrows;
-                int slot_k = s;
-                wait(full0 + 8 * slot_k, parity);
-                wait(qfull, qparity);
+            auto wait = [&](uint32_t bar, uint32_t par) {
+                if (ok) ok = wait_here(bar, par);
+            };
+            for (int taken; (taken = c.run<PrefillRuns>()) > 0;) {
+                const uint32_t run = __reduce_max_sync(0xffffffffu, (uint32_t)taken), two = __reduce_max_sync(0xffffffffu, c.s.rows > qrows ? 1u : 0u);
+                wait(full0 + 8 * (n % S::SLOTS), (n / S::SLOTS) & 1u);
+                wait(qfull, items & 1u);
                 tc_fence_after();
-                qparity ^= 1u;
-                next_slot();
-                if (!failed && elect_one()) {
-                    scores(0, slot_k);
+                if (!ok) break;
+                if (lead) {
+                    scores(0, n % S::SLOTS);
                     umma_commit(sfull0);
-                    if (two) scores(1, slot_k), umma_commit(sfull0 + 8);
-                    umma_commit(empty0 + 8 * slot_k);
+                    if (two) scores(1, n % S::SLOTS), umma_commit(sfull0 + 8);
+                    umma_commit(empty0 + 8 * (n % S::SLOTS));
                     if (run == 1) umma_commit(qempty);
                 }
                 __syncwarp();
-                for (int i = 0; i < run; ++i) {
-                    const int slot_v = s;
-                    wait(full0 + 8 * slot_v, parity);
-                    wait(clean0 + 8 * slot_v, parity);
-                    next_slot();
-                    const bool more = i + 1 < run;
-                    slot_k = s;
-                    wait(pfull0, pparity0);
+                ++n, ++items;
+                for (uint32_t i = 0; i < run && ok; ++i) {
+                    const uint32_t sv = n % S::SLOTS, sk = (n + 1) % S::SLOTS, pv = (n / S::SLOTS) & 1u, pk = ((n + 1) / S::SLOTS) & 1u, more = i + 1 < run, acc = i != 0;
+                    wait(full0 + 8 * sv, pv);
+                    wait(clean0 + 8 * sv, pv);
+                    wait(pfull0, p0);
                     tc_fence_after();
-                    if (!failed && elect_one()) values(0, slot_v, 0, i == 0);
+                    if (lead && ok) values(0, sv, 0, acc);
                     __syncwarp();
-                    if (more) {
-                        wait(full0 + 8 * slot_k, parity);
-                        next_slot();
-                    }
-                    wait(phalf0, pparity0);
+                    if (more) wait(full0 + 8 * sk, pk);
+                    wait(phalf0, p0);
                     tc_fence_after();
-                    pparity0 ^= 1u;
-                    if (!failed && elect_one()) {
-                        values(0, slot_v, 1, i == 0);
-                        if (more) scores(0, slot_k);
+                    p0 ^= 1u;
+                    if (lead && ok) {
+                        values(0, sv, 1, acc);
+                        if (more) scores(0, sk);
                         umma_commit(sfull0);                                 // S0 of the next tile is there, O0 of this one too
                     }
                     __syncwarp();
                     if (two) {
-                        wait(pfull0 + 8, pparity1);
+                        wait(pfull0 + 8, p1);
                         tc_fence_after();
-                        if (!failed && elect_one()) values(1, slot_v, 0, i == 0);
+                        if (lead && ok) values(1, sv, 0, acc);
                         __syncwarp();
-                        wait(phalf0 + 8, pparity1);
+                        wait(phalf0 + 8, p1);
                         tc_fence_after();
-                        pparity1 ^= 1u;
-                        if (!failed && elect_one()) {
-                            values(1, slot_v, 1, i == 0);
-                            umma_commit(empty0 + 8 * slot_v);
-                            if (more) scores(1, slot_k);
-                            umma_commit(sfull0 + 8);
-                            if (more) umma_commit(empty0 + 8 * slot_k);
-                            if (i + 2 == run) umma_commit(qempty);
-                        }
-                    } else if (!failed && elect_one()) {
-                        umma_commit(empty0 + 8 * slot_v);
-                        if (more) umma_commit(empty0 + 8 * slot_k);
+                        p1 ^= 1u;
+                    }
+                    if (lead && ok) {
+                        if (two) values(1, sv, 1, acc);
+                        umma_commit(empty0 + 8 * sv);
+                        if (two && more) scores(1, sk);
+                        if (two) umma_commit(sfull0 + 8);
+                        if (more) umma_commit(empty0 + 8 * sk);
                         if (i + 2 == run) umma_commit(qempty);
                     }
                     __syncwarp();
+                    n += 1 + more;
                 }
-                c.advance<PrefillRuns>(p, block, PF_TILE, run);
+                c.advance<PrefillRuns>(p, block, PF_TILE, taken);
             }
+            failed = !ok;
         } else if (warp == 10) {
             // ---- between producer and issuer: values in places that no row sees become 0 (the first and last tiles of an item)
             int s = 1;
@@ -540,12 +535,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_attn_prefill_kernel(const
                                          : "memory");
                     }
                     __syncwarp();
+                    uint4 y[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) y[k] = lds128(stage + (4 * k + (lane >> 3)) * 128 + (((lane & 7) ^ ((4 * k + (lane >> 3)) & 7)) << 4));
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        const int r = 4 * k + (lane >> 3);
-                        uint8_t* const to_row = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), r));
-                        const uint4 y = lds128(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-                        if (to_row) *reinterpret_cast<uint4*>(to_row + off + (lane & 7) * 16) = y;
+                        uint8_t* const to_row = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), 4 * k + (lane >> 3)));
+                        if (to_row) *reinterpret_cast<uint4*>(to_row + off + (lane & 7) * 16) = y[k];
                     }
                 }
                 tc_fence_before();
@@ -602,6 +598,7 @@ int launch_prefill(KybAttnCall& c, void* ws) {
     auto kern = kyb::paged_attn_prefill_kernel<T, D>;
     if (int rc = kyb_allow_smem((const void*)kern)) return rc;
     const int ctas = c.sms, piece = std::min(c.page, kyb::PF_TILE), qtoks = 128 / c.p.group;
+    KYB_REQUIRE(kyb_attn_units_fit(c, 2 * qtoks * c.p.group, kyb::PF_TILE), "more than 2^31 key tiles in one call: split it");
     CUtensorMap mq, mk, mv;
     if (int rc = make_query_map(&mq, c, qtoks)) return rc;
     if (int rc = kyb_make_cache_map(&mk, c.k, c.dtype, c.p.pages, c.p.hkv, c.page, D, c.k_p, c.k_h, piece, 1)) return rc;
