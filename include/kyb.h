@@ -251,7 +251,8 @@ int kyb_gemv_t16_static(int fmt, const void* t16, int64_t n, int64_t k, const vo
 /* ---- paged key/value cache: the part of a decoder layer between its q|k|v product and its o product. No counterpart in the reference's quantized-linear path.
  * Cache layout: [page][kv head][token of the page][value], 16-bit values, strides of pages and heads in elements (multiples of 8), 16-byte aligned; tokens of a
  * page 16 to 256, a power of two. A request's tokens lie in the pages of its row of `table` (int32 [batch, cols], row stride ld_table), in order; a slot is
- * page id * tokens of a page + place in the page. dtype: 1 fp16, 2 bf16. Integer arrays are int32 on the device.
+ * page id * tokens of a page + place in the page. dtype: 1 fp16, 2 bf16. Integer arrays are int32 on the device. Arguments come as one block of 8-byte fields (host
+ * memory, read before the call returns): a decode step makes these calls for every layer, and a host language passes a block in a fifth of the time of 30 arguments.
  *
  * kyb_paged_step: slots of a step from request lengths. Request r holds lens[r] tokens and brings new_lens[r] (negative values count as 0); pages it lacks come from
  * the top of free_pages[0, *free_count) (an array of free_cap ids), in request order, and are entered in its row of table. A request is served when its pages fit
@@ -259,9 +260,12 @@ int kyb_gemv_t16_static(int fmt, const void* t16, int64_t n, int64_t k, const vo
  * Out: cu_q [batch + 1] first row of each request (clipped to rows), kv_lens [batch] tokens to attend over (0: not served), positions [rows] and slots [rows] (-1:
  * not served, or a row behind the last request), lens_out [batch] (may be lens), free_count_out [1] (may be free_count), refused [1] number not served. The entries of
  * free_pages and of the table's other columns stay as they are: the same call again gives the same result unless lens_out / free_count_out are the inputs. */
-int kyb_paged_step(const void* lens, const void* new_lens, const void* free_pages, int64_t free_cap, const void* free_count, void* table, int64_t ld_table,
-                   int64_t batch, int64_t cols, int page, int64_t rows, void* cu_q, void* kv_lens, void* positions, void* slots, void* lens_out,
-                   void* free_count_out, void* refused, void* stream);
+typedef struct {
+    const void *lens, *new_lens, *free_pages, *free_count;
+    void *table, *cu_q, *kv_lens, *positions, *slots, *lens_out, *free_count_out, *refused;
+    int64_t free_cap, ld_table, batch, cols, page, rows;
+} kyb_paged_step_args;
+int kyb_paged_step(const kyb_paged_step_args* args, void* stream);
 /* pages of the requests with which[r] != 0 (uint8 [batch]) go back to the free list; their table entries become -1, their lengths 0. A request whose pages would
  * overflow the list keeps them and is counted in refused [1]. */
 int kyb_paged_release(void* lens, const void* which, void* table, int64_t ld_table, int64_t batch, int64_t cols, int page, void* free_pages, int64_t free_cap,
@@ -270,10 +274,15 @@ int kyb_paged_release(void* lens, const void* which, void* table, int64_t ld_tab
  * positions[t] * inv_freq[i] (fp32 [rot / 2]; product and reduction in 64 bits) and scaled by mscale; queries to q_out (may be q), keys and values to the cache at
  * slots[t]. A row with positions[t] < 0 is left alone, a slot outside the cache stores nothing. hkv = 0: queries only. d a multiple of 8 up to 256, rot a
  * multiple of 16. Strides in elements. Slots that two rows share hold one of them in the end. */
-int kyb_rope_append(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_t, int64_t k_h, const void* v, int64_t v_t, int64_t v_h,
-                    const void* positions, const void* slots, const void* inv_freq, int64_t tokens, int hq, int hkv, int d, int rot, int interleaved,
-                    float mscale, int dtype, void* q_out, int64_t qo_t, int64_t qo_h, void* k_cache, int64_t kc_page, int64_t kc_head, void* v_cache,
-                    int64_t vc_page, int64_t vc_head, int64_t pages, int page, void* stream);
+typedef struct {
+    const void *q, *k, *v, *positions, *slots, *inv_freq;
+    void *q_out, *k_cache, *v_cache;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head, q_out_token, q_out_head;    /* strides */
+    int64_t k_cache_page, k_cache_head, v_cache_page, v_cache_head;
+    int64_t tokens, hq, hkv, d, rot, interleaved, dtype, pages, page;
+    double mscale;
+} kyb_rope_append_args;
+int kyb_rope_append(const kyb_rope_append_args* args, void* stream);
 /* attention of a step's new tokens over the cache: request r owns the rows [cu_q[r], cu_q[r + 1]) of q and out ([tokens][hq][d]), its last row is its token
  * kv_lens[r] - 1. The token at position p sees key j when j <= p and, with window > 0, j > p - window or j < sinks. A row that sees nothing gives zeros; rows outside
  * [cu_q[0], cu_q[batch]) stay as they are. max_q: the largest number of rows of a request (it chooses the kernel; rows of longer requests are served too).
@@ -281,10 +290,14 @@ int kyb_rope_append(const void* q, int64_t q_t, int64_t q_h, const void* k, int6
  * may hold anything. Other places must hold finite values. Scores, sums and the output's accumulation in 32 bits; the weights enter the product with V in the
  * inputs' type, as the tensor cores take them. Scratch: kyb_paged_attention_workspace_bytes, private to the call until it has run. */
 size_t kyb_paged_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t max_q, int64_t cols, int page, int hq, int hkv, int d);
-int kyb_paged_attention(const void* q, int64_t q_t, int64_t q_h, const void* k_cache, int64_t k_page, int64_t k_head, const void* v_cache, int64_t v_page,
-                        int64_t v_head, int64_t pages, int page, const void* table, int64_t ld_table, int64_t cols, const void* kv_lens, const void* cu_q,
-                        int64_t batch, int64_t tokens, int64_t max_q, int hq, int hkv, int d, int dtype, float scale, int64_t window, int64_t sinks, void* out,
-                        int64_t o_t, int64_t o_h, void* ws, size_t ws_bytes, void* stream);
+typedef struct {
+    const void *q, *k_cache, *v_cache, *table, *kv_lens, *cu_q;
+    void *out, *ws;
+    int64_t q_token, q_head, k_page, k_head, v_page, v_head, out_token, out_head;          /* strides */
+    int64_t pages, page, ld_table, cols, batch, tokens, max_q, hq, hkv, d, dtype, window, sinks, ws_bytes;
+    double scale;
+} kyb_paged_attention_args;
+int kyb_paged_attention(const kyb_paged_attention_args* args, void* stream);
 
 /* launch plan the GEMV would use (diagnostics): out8 = {column tiles, how work is dealt (1: whole row tiles per warp, one launch; 0: runs of chunks per warp,
  * chunk sums through the workspace and a finalize launch; 2: whole row tiles per CTA, chunk sums added in shared memory, one launch), warps per CTA, k-blocks

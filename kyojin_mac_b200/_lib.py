@@ -7,6 +7,7 @@ from __future__ import annotations
 import ctypes as C
 import glob
 import os
+import struct
 import subprocess
 import threading
 
@@ -109,6 +110,12 @@ class PeerOut(C.Structure):
 
 
 _pp = C.POINTER(PeerOut)
+
+# argument blocks of the paged-cache entries (kyb_*_args): pointers, then int64 fields, then a double where there is one; packed by struct in native order
+PAGED_STEP_ARGS = struct.Struct("=12Q6q")
+ROPE_APPEND_ARGS = struct.Struct("=9Q21qd")
+PAGED_ATTENTION_ARGS = struct.Struct("=8Q22qd")
+
 SIGNATURES = {
     "kyb_version": (_int, []),
     "kyb_status_string": (C.c_char_p, [_int]),
@@ -160,12 +167,11 @@ SIGNATURES = {
     "kyb_gemv_group_t16": (_int, [_int, _vp, _vp, _i64, _i64, _int, _vp, _vp, _f32, _i64, _vp, _vp, _int, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp]),
     "kyb_gemv_plan": (_int, [_int, _i64, _i64, _i64, C.POINTER(C.c_int)]),
     "kyb_gemv_plan_within": (_int, [_int, _i64, _i64, _i64, _sz, C.POINTER(C.c_int)]),
-    "kyb_paged_step": (_int, [_vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _int, _i64] + [_vp] * 8),
+    "kyb_paged_step": (_int, [C.c_char_p, _vp]),
     "kyb_paged_release": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _i64, _vp, _vp, _vp]),
-    "kyb_rope_append": (_int, [_vp, _i64, _i64] * 3 + [_vp, _vp, _vp, _i64, _int, _int, _int, _int, _int, _f32, _int] + [_vp, _i64, _i64] * 3 + [_i64, _int, _vp]),
+    "kyb_rope_append": (_int, [C.c_char_p, _vp]),
     "kyb_paged_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _int, _int, _int, _int]),
-    "kyb_paged_attention": (_int, [_vp, _i64, _i64] * 3 + [_i64, _int, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _int, _int, _int, _int, _f32, _i64, _i64] + [_vp, _i64, _i64]
-                            + [_vp, _sz, _vp]),
+    "kyb_paged_attention": (_int, [C.c_char_p, _vp]),
     "kyb_check_device_status": (_int, [_vp]),
     "kyb_selftest_wait_timeout": (_int, [_int, _vp]),
 }

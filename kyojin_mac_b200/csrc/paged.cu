@@ -283,9 +283,13 @@ __global__ void __launch_bounds__(RP_THREADS) rope_append_kernel(const RopeParam
 
 }  // namespace kyb
 
-extern "C" int kyb_paged_step(const void* lens, const void* new_lens, const void* free_pages, int64_t free_cap, const void* free_count, void* table, int64_t ld_table, int64_t batch,
-                              int64_t cols, int page, int64_t rows, void* cu_q, void* kv_lens, void* positions, void* slots, void* lens_out, void* free_count_out, void* refused,
-                              void* stream) {
+extern "C" int kyb_paged_step(const kyb_paged_step_args* a, void* stream) {
+    KYB_REQUIRE(a, "null pointer");
+    const void *lens = a->lens, *new_lens = a->new_lens, *free_pages = a->free_pages, *free_count = a->free_count;
+    void *table = a->table, *cu_q = a->cu_q, *kv_lens = a->kv_lens, *positions = a->positions, *slots = a->slots, *lens_out = a->lens_out, *free_count_out = a->free_count_out,
+         *refused = a->refused;
+    const int64_t free_cap = a->free_cap, ld_table = a->ld_table, batch = a->batch, cols = a->cols, rows = a->rows;
+    const int page = (int)std::min<int64_t>(std::max<int64_t>(a->page, 0), 1 << 20);
     KYB_REQUIRE(lens && new_lens && free_pages && free_count && table && cu_q && kv_lens && lens_out && free_count_out && refused && (rows == 0 || (positions && slots)), "null pointer");
     KYB_REQUIRE(batch > 0 && batch < (1ll << 24) && cols > 0 && ld_table >= cols && rows >= 0 && rows < (1ll << 31) && free_cap > 0 && free_cap < (1ll << 31),
                 "batch=%lld cols=%lld (row stride %lld) rows=%lld free list of %lld: out of range", (long long)batch, (long long)cols, (long long)ld_table, (long long)rows,
@@ -318,25 +322,31 @@ extern "C" int kyb_paged_release(void* lens, const void* which, void* table, int
     return kyb_launch_check("paged_release");
 }
 
-extern "C" int kyb_rope_append(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_t, int64_t k_h, const void* v, int64_t v_t, int64_t v_h, const void* positions,
-                               const void* slots, const void* inv_freq, int64_t tokens, int hq, int hkv, int d, int rot, int interleaved, float mscale, int dtype, void* q_out,
-                               int64_t qo_t, int64_t qo_h, void* k_cache, int64_t kc_page, int64_t kc_head, void* v_cache, int64_t vc_page, int64_t vc_head, int64_t pages, int page,
-                               void* stream) {
-    KYB_REQUIRE(tokens >= 0 && tokens < (1ll << 31) && hq >= 0 && hkv >= 0 && hq + hkv > 0 && hq <= 65536 && hkv <= 65536, "tokens=%lld heads %d + %d: out of range", (long long)tokens,
+extern "C" int kyb_rope_append(const kyb_rope_append_args* a, void* stream) {
+    KYB_REQUIRE(a, "null pointer");
+    const void *q = a->q, *k = a->k, *v = a->v, *positions = a->positions, *slots = a->slots, *inv_freq = a->inv_freq;
+    void *q_out = a->q_out, *k_cache = a->k_cache, *v_cache = a->v_cache;
+    const int64_t tokens = a->tokens, pages = a->pages;
+    for (int64_t n : {a->hq, a->hkv, a->d, a->rot, a->dtype, a->page}) KYB_REQUIRE(n >= 0 && n <= 65536, "a size of %lld: out of range", (long long)n);
+    const int hq = (int)a->hq, hkv = (int)a->hkv, d = (int)a->d, rot = (int)a->rot, dtype = (int)a->dtype, page = (int)a->page;
+    const bool interleaved = a->interleaved != 0;
+    const float mscale = (float)a->mscale;
+    KYB_REQUIRE(tokens >= 0 && tokens < (1ll << 31) && hq + hkv > 0, "tokens=%lld heads %d + %d: out of range", (long long)tokens,
                 hq, hkv);
     KYB_REQUIRE(d >= 16 && d <= 256 && d % 8 == 0 && rot >= 16 && rot <= d && rot % 16 == 0, "d=%d rot=%d: d a multiple of 8 up to 256, rot a multiple of 16 from 16 to d", d, rot);
     KYB_REQUIRE(dtype == 1 || dtype == 2, "dtype=%d: 1 (fp16) or 2 (bf16)", dtype);
     if (tokens == 0) return KYB_OK;
     KYB_REQUIRE(positions && inv_freq && (hq == 0 || (q && q_out)) && (hkv == 0 || (k && v && slots && k_cache && v_cache)), "null pointer");
-    const int64_t strides[] = {q_t, q_h, k_t, k_h, v_t, v_h, qo_t, qo_h, kc_page, kc_head, vc_page, vc_head};
-    for (int64_t s : strides) KYB_REQUIRE(s % 8 == 0, "a stride of %lld elements: strides are multiples of 8 elements (16 bytes)", (long long)s);
+    for (int64_t s : {a->q_token, a->q_head, a->k_token, a->k_head, a->v_token, a->v_head, a->q_out_token, a->q_out_head, a->k_cache_page, a->k_cache_head, a->v_cache_page, a->v_cache_head})
+        KYB_REQUIRE(s % 8 == 0, "a stride of %lld elements: strides are multiples of 8 elements (16 bytes)", (long long)s);
     KYB_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) == 0, "pointers must be 16-byte aligned");
     KYB_REQUIRE(hkv == 0 || (page >= 16 && page <= 256 && (page & (page - 1)) == 0 && pages > 0 && pages < (1ll << 31)), "page=%d pages=%lld: a power of two from 16 to 256, at least one page",
                 page, (long long)pages);
     kyb::RopeParams p;
     p.q = (const uint8_t*)q, p.k = (const uint8_t*)k, p.v = (const uint8_t*)v, p.qo = (uint8_t*)q_out, p.kc = (uint8_t*)k_cache, p.vc = (uint8_t*)v_cache;
-    p.q_t = q_t * 2, p.q_h = q_h * 2, p.k_t = k_t * 2, p.k_h = k_h * 2, p.v_t = v_t * 2, p.v_h = v_h * 2, p.qo_t = qo_t * 2, p.qo_h = qo_h * 2;
-    p.kc_p = kc_page * 2, p.kc_h = kc_head * 2, p.vc_p = vc_page * 2, p.vc_h = vc_head * 2;
+    p.q_t = a->q_token * 2, p.q_h = a->q_head * 2, p.k_t = a->k_token * 2, p.k_h = a->k_head * 2, p.v_t = a->v_token * 2, p.v_h = a->v_head * 2;
+    p.qo_t = a->q_out_token * 2, p.qo_h = a->q_out_head * 2;
+    p.kc_p = a->k_cache_page * 2, p.kc_h = a->k_cache_head * 2, p.vc_p = a->v_cache_page * 2, p.vc_h = a->v_cache_head * 2;
     p.positions = (const int*)positions, p.slots = (const int*)slots, p.inv = (const float*)inv_freq, p.pages = pages;
     p.page_log2 = 0;
     while (hkv && (1 << p.page_log2) < page) ++p.page_log2;

@@ -184,6 +184,21 @@ static inline int kyb_make_cache_map(CUtensorMap* tm, const void* base, int dtyp
     return KYB_OK;
 }
 
+#ifdef __CUDACC__
+// launch whose beginning may overlap the end of the kernel before it on the stream (the kernel waits for that one before it reads or writes memory)
+template <typename K, typename... A>
+static inline int kyb_launch_chained(K kern, int ctas, int threads, size_t smem, cudaStream_t st, const A&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas), cfg.blockDim = dim3((unsigned)threads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at, cfg.numAttrs = 1;
+    KYB_CUDA(cudaLaunchKernelEx(&cfg, kern, args...));
+    return KYB_OK;
+}
+#endif
+
 // The call as the C entry hands it to a kernel's launcher
 struct KybAttnCall {
     kyb::AttnParams p;

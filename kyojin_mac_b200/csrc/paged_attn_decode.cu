@@ -116,6 +116,7 @@ __global__ void __launch_bounds__(DC_THREADS, 2) paged_attn_decode_kernel(const 
         prefetch_tmap(&map_k);
         prefetch_tmap(&map_v);
     }
+    pdl_wait();                                                              // what is above runs while the kernel before drains
     find_run(p, S::ROWS, &start, sums, DC_THREADS);
     Cursor c = start;
     pdl_launch_dependents();
@@ -354,9 +355,11 @@ constexpr int JOIN_ROWS = 8;
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * JOIN_ROWS) paged_attn_join_kernel(const AttnParams p, const int ctas, const int block) {
     constexpr int E = D / 32;
+    pdl_launch_dependents();
     pdl_wait();
-    const int first = blockIdx.x, lane = threadIdx.x & 31, rr = blockIdx.y * JOIN_ROWS + (threadIdx.x >> 5);
+    const int first = blockIdx.x, lane = threadIdx.x & 31;
     const int4 note = p.notes[first];
+    const int rr = blockIdx.y * JOIN_ROWS + (threadIdx.x >> 5);
     if (!(note.w & NOTE_BEGINS) || rr >= block) return;
     int row_base;
     const int tokens = request_rows(p, note.x, row_base), row = note.y * block + rr, tok = row / p.group;
@@ -422,8 +425,7 @@ int launch_decode(KybAttnCall& c, void* ws) {
     if (int rc = kyb_make_cache_map(&mk, c.k, c.dtype, c.p.pages, c.p.hkv, c.page, D, c.k_p, c.k_h, piece, D / 64)) return rc;
     if (int rc = kyb_make_cache_map(&mv, c.v, c.dtype, c.p.pages, c.p.hkv, c.page, D, c.v_p, c.v_h, piece, D / 64)) return rc;
     c.p.notes = (int4*)ws, c.p.parts = (float*)((char*)ws + (size_t)ctas * sizeof(int4));
-    kern<<<(unsigned)ctas, kyb::DC_THREADS, S::SMEM + 1024, c.st>>>(mk, mv, c.p);
-    if (int rc = kyb_launch_check("paged_attn_decode")) return rc;
+    if (int rc = kyb_launch_chained(kern, ctas, kyb::DC_THREADS, S::SMEM + 1024, c.st, mk, mv, c.p)) return rc;
     return kyb_attn_join(c, ctas, S::ROWS);
 }
 

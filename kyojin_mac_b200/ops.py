@@ -540,6 +540,18 @@ def _cache(t, name, like=None):
         raise ValueError(f"{name}: the tokens of a page and head must be dense, strides multiples of 8 elements, the start 16-byte aligned; got strides {t.stride()}")
 
 
+# Calls whose shapes, strides, types and numbers have passed the checks (their description; nothing of their data): a decode step repeats its calls for every layer and
+# token, and the checks cost more than the launch.
+_passed: dict = {}
+
+
+def _remember(key, value):
+    if len(_passed) >= 1024:
+        _passed.clear()
+    _passed[key] = value
+    return value
+
+
 class PagedStep(NamedTuple):
     """What `paged_step` gives: int32 device tensors."""
     cu_q: torch.Tensor          # [batch + 1] first row of each request
@@ -557,21 +569,29 @@ def paged_step(table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor, 
     into the step's `rows` rows); the pages it lacks come from the top of free_pages[:free_count] and are entered in its row of `table` [batch, columns].
     A request is served when its pages fit the columns, its tokens the rows, and the needs of the requests up to its own the free list (one that needs no page
     is not held up); `refused` counts the others, whose lengths stay. in_place: lens and free_count are updated too (a captured step that is replayed)."""
-    guard = _place(table, lens, new_lens, free_pages, free_count)
-    _table(table, page)
-    b, cols = table.shape
-    _i32(lens, "lens", b), _i32(new_lens, "new_lens", b), _i32(free_pages, "free_pages", None), _i32(free_count, "free_count", 1)
-    if free_pages.numel() < 1 or rows < 0:
-        raise ValueError("the free list is an array with room for a page at least, rows not negative")
-    with guard:
+    dev = table.get_device()
+    key = (dev, table.shape, table.stride(), table.dtype, lens.shape, lens.dtype, lens.is_contiguous(), new_lens.shape, new_lens.dtype, new_lens.is_contiguous(), free_pages.shape, free_pages.dtype,
+           free_pages.is_contiguous(), free_count.shape, free_count.dtype, page, rows, in_place, lens.get_device(), new_lens.get_device(), free_pages.get_device(), free_count.get_device())
+    known = _passed.get(key)
+    if known is None:
+        _place(table, lens, new_lens, free_pages, free_count)
+        _table(table, page)
+        b, cols = table.shape
+        _i32(lens, "lens", b), _i32(new_lens, "new_lens", b), _i32(free_pages, "free_pages", None), _i32(free_count, "free_count", 1)
+        if free_pages.numel() < 1 or rows < 0:
+            raise ValueError("the free list is an array with room for a page at least, rows not negative")
         sizes = [b + 1, b, rows, rows, 1] + ([] if in_place else [b, 1])
-        cu, kv, pos, slots, refused, *more = lens.new_empty(sum(sizes)).split_with_sizes(sizes)
-        out_lens, out_count = (lens, free_count) if in_place else more
-        rc = _lib.lib().kyb_paged_step(lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), table.data_ptr(), max(table.stride(0), cols), b,
-                                       cols, page, rows, cu.data_ptr(), kv.data_ptr(), pos.data_ptr(), slots.data_ptr(), out_lens.data_ptr(), out_count.data_ptr(), refused.data_ptr(),
-                                       _stream())
-        if rc:
-            _lib.check(rc)
+        known = _remember(key, (sum(sizes), sizes, (free_pages.shape[0], max(table.stride(0), cols), b, cols, page, rows)))
+    if dev != torch.cuda.current_device() if _cur_device is None else dev != _cur_device():
+        with torch.cuda.device(dev):
+            return paged_step(table, lens, new_lens, free_pages, free_count, page, rows, in_place)
+    total, sizes, numbers = known
+    cu, kv, pos, slots, refused, *more = lens.new_empty(total).split_with_sizes(sizes)
+    out_lens, out_count = (lens, free_count) if in_place else more
+    rc = _lib.lib().kyb_paged_step(_lib.PAGED_STEP_ARGS.pack(lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), table.data_ptr(), cu.data_ptr(), kv.data_ptr(),
+                                                             pos.data_ptr(), slots.data_ptr(), out_lens.data_ptr(), out_count.data_ptr(), refused.data_ptr(), *numbers), _stream())
+    if rc:
+        _lib.check(rc)
     return PagedStep(cu, kv, pos, slots, out_lens, out_count, refused)
 
 
@@ -629,26 +649,54 @@ def rope_frequencies(rot: int, base: float = 10000.0, scaling: dict | None = Non
     return inv.to(torch.float32).to(device), mscale
 
 
-def _rope_call(q, k, v, positions, slots, inv_freq, kc, vc, interleaved, mscale, out):
+def _rope_check(key, q, k, v, positions, slots, inv_freq, kc, vc, out):
+    _place(*(t for t in (q, k, v, positions, slots, inv_freq, kc, vc, out) if t is not None))
+    _heads(q, "q"), _i32(positions, "positions", q.shape[0])
     if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq is contiguous float32 [rot / 2]")
     T, hq, d = q.shape
-    if out is None:
-        out = q.new_empty((T, hq, d))
-    else:
+    if out is not None:
         _heads(out, "out")
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError("out has the queries' shape and type")
-    qs, os_, zero = q.stride(), out.stride(), (None, 0, 0)
-    kp, vp, kcp, vcp = zero, zero, zero, zero
+    ks = vs = kcs = vcs = (0, 0)
     hkv = pages = page = 0
     if k is not None:
-        ks, vs, kcs, vcs = k.stride(), v.stride(), kc.stride(), vc.stride()
+        _heads(k, "k"), _heads(v, "v"), _cache(kc, "k_cache"), _cache(vc, "v_cache", kc), _i32(slots, "slots", T)
+        if k.shape != (T, kc.shape[1], d) or v.shape != k.shape or kc.shape[3] != d or not q.dtype == k.dtype == v.dtype == kc.dtype:
+            raise ValueError(f"q [T, heads, d], k and v [T, kv heads, d] and the cache go together, in one type: got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}, {tuple(kc.shape)}")
+        ks, vs, kcs, vcs = k.stride()[:2], v.stride()[:2], kc.stride()[:2], vc.stride()[:2]
         pages, hkv, page = kc.shape[:3]
-        kp, vp = (k.data_ptr(), ks[0], ks[1]), (v.data_ptr(), vs[0], vs[1])
-        kcp, vcp = (kc.data_ptr(), kcs[0], kcs[1]), (vc.data_ptr(), vcs[0], vcs[1])
-    rc = _lib.lib().kyb_rope_append(q.data_ptr(), qs[0], qs[1], *kp, *vp, positions.data_ptr(), None if slots is None else slots.data_ptr(), inv_freq.data_ptr(), T, hq, hkv, d,
-                                    2 * inv_freq.shape[0], 1 if interleaved else 0, mscale, _DT[q.dtype], out.data_ptr(), os_[0], os_[1], *kcp, *vcp, pages, page, _stream())
+    os_ = (hq * d, d) if out is None else out.stride()[:2]
+    return _remember(key, (*q.stride()[:2], *ks, *vs, *os_, *kcs, *vcs, T, hq, hkv, d, 2 * inv_freq.shape[0]))
+
+
+def _rope_call(q, k, v, positions, slots, inv_freq, kc, vc, interleaved, mscale, out):
+    """The queries turned (into `out`), keys and values into the cache where there are any."""
+    dev, grad = q.get_device(), q.requires_grad
+    if k is None:
+        key = (dev, q.shape, q.stride(), q.dtype, positions.shape, positions.dtype, positions.is_contiguous(), inv_freq.shape, inv_freq.dtype, positions.get_device(), inv_freq.get_device())
+    else:
+        grad = grad or k.requires_grad or v.requires_grad
+        key = (dev, q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, positions.shape, positions.dtype, positions.is_contiguous(), slots.shape, slots.dtype,
+               slots.is_contiguous(), inv_freq.shape, inv_freq.dtype, kc.shape, kc.stride(), kc.dtype, vc.shape, vc.stride(), vc.dtype, k.get_device(), v.get_device(), positions.get_device(),
+               slots.get_device(), inv_freq.get_device(), kc.get_device(), vc.get_device())
+    if out is not None:
+        key += (out.shape, out.stride(), out.dtype, out.get_device())
+    sizes = None if grad or not inv_freq.is_contiguous() else _passed.get(key)
+    if sizes is None:
+        sizes = _rope_check(key, q, k, v, positions, slots, inv_freq, kc, vc, out)
+    if dev != torch.cuda.current_device() if _cur_device is None else dev != _cur_device():
+        with torch.cuda.device(dev):
+            return _rope_call(q, k, v, positions, slots, inv_freq, kc, vc, interleaved, mscale, out)
+    if out is None:
+        out = q.new_empty(q.shape)
+    if k is None:
+        ptrs, pages = (q.data_ptr(), 0, 0, positions.data_ptr(), 0, inv_freq.data_ptr(), out.data_ptr(), 0, 0), (0, 0)
+    else:
+        ptrs = (q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr(), out.data_ptr(), kc.data_ptr(), vc.data_ptr())
+        pages = kc.shape[0], kc.shape[2]
+    rc = _lib.lib().kyb_rope_append(_lib.ROPE_APPEND_ARGS.pack(*ptrs, *sizes, 1 if interleaved else 0, _DT[q.dtype], *pages, mscale), _stream())
     if rc:
         _lib.check(rc)
     return out
@@ -657,10 +705,7 @@ def _rope_call(q, k, v, positions, slots, inv_freq, kc, vc, interleaved, mscale,
 def rope(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False, mscale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
     """x fp16 / bf16 [tokens, heads, d] with the first rot = 2 len(inv_freq) values of every head turned: pairs (i, i + rot / 2), or (2 i, 2 i + 1) when interleaved, by
     positions[t] * inv_freq[i], scaled by mscale. Rows of a negative position are left as they are in `out` (which may be x)."""
-    guard = _place(x, positions, inv_freq, *(() if out is None else (out,)))
-    _heads(x, "x"), _i32(positions, "positions", x.shape[0])
-    with guard:
-        return _rope_call(x, None, None, positions, None, inv_freq, None, None, interleaved, float(mscale), out)
+    return _rope_call(x, None, None, positions, None, inv_freq, None, None, interleaved, mscale, out)
 
 
 def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, inv_freq: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -668,14 +713,29 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     """`rope` of a step's queries, and in the same launch its keys (turned) and values into the cache [pages, kv heads, tokens of a page, d] at slots[t]. q [T, heads, d],
     k and v [T, kv heads, d] may be views of one q | k | v product. Returns the turned queries. Rows with a negative position are left alone, a slot outside the cache
     stores nothing; of rows that share a slot one is stored."""
-    guard = _place(q, k, v, positions, slots, inv_freq, k_cache, v_cache, *(() if out is None else (out,)))
-    _heads(q, "q"), _heads(k, "k"), _heads(v, "v"), _cache(k_cache, "k_cache"), _cache(v_cache, "v_cache", k_cache)
-    T, d = q.shape[0], q.shape[2]
-    if k.shape != (T, k_cache.shape[1], d) or v.shape != k.shape or k_cache.shape[3] != d or not q.dtype == k.dtype == v.dtype == k_cache.dtype:
-        raise ValueError(f"q [T, heads, d], k and v [T, kv heads, d] and the cache go together, in one type: got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}, {tuple(k_cache.shape)}")
-    _i32(positions, "positions", T), _i32(slots, "slots", T)
-    with guard:
-        return _rope_call(q, k, v, positions, slots, inv_freq, k_cache, v_cache, interleaved, float(mscale), out)
+    return _rope_call(q, k, v, positions, slots, inv_freq, k_cache, v_cache, interleaved, mscale, out)
+
+
+def _attention_check(key, q, kc, vc, table, kv_lens, cu_q, max_q, window, sinks, out):
+    _place(*(t for t in (q, kc, vc, table, kv_lens, cu_q, out) if t is not None))
+    _heads(q, "q"), _cache(kc, "k_cache"), _cache(vc, "v_cache", kc)
+    (T, hq, d), (pages, hkv, page, dk) = q.shape, kc.shape
+    _table(table, page)
+    b, cols = table.shape
+    _i32(kv_lens, "kv_lens", b), _i32(cu_q, "cu_q", b + 1)
+    if d != dk or d not in (64, 128) or q.dtype != kc.dtype or hq % hkv or hq < hkv:
+        raise ValueError(f"heads of 64 or 128, a multiple of the cache's heads, in the cache's type: got q {q.dtype} {tuple(q.shape)}, cache {kc.dtype} {tuple(kc.shape)}")
+    if max_q < 0 or window < 0 or sinks < 0 or (sinks and not window):
+        raise ValueError("max_q, window and sinks are not negative, sinks come with a window")
+    if out is not None:
+        _heads(out, "out")
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError("out has the queries' shape and type")
+    with torch.cuda.device(q.device):
+        need = _lib.lib().kyb_paged_attention_workspace_bytes(b, T, max_q, cols, page, hq, hkv, d)
+    os_ = (hq * d, d) if out is None else out.stride()[:2]
+    return _remember(key, (need, (*q.stride()[:2], *kc.stride()[:2], *vc.stride()[:2], *os_, pages, page, max(table.stride(0), cols), cols, b, T, max_q, hq, hkv, d, _DT[q.dtype], window, sinks,
+                                  need)))
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, kv_lens: torch.Tensor, cu_q: torch.Tensor, max_q: int, scale: float | None = None,
@@ -684,30 +744,22 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     kv_lens[r] - 1), keys and values through the block table [batch, columns]. Causal; window > 0: the last `window` tokens only, and the first `sinks` ones.
     max_q: the largest number of new tokens of a request (chooses the kernel; requests with more are served all the same). scale: d ** -0.5 unless given.
     A row that sees nothing (kv_lens 0) gives zeros; rows behind the last request are left as they were (undefined without `out`). Returns out [T, heads, d]."""
-    guard = _place(q, k_cache, v_cache, table, kv_lens, cu_q, *(() if out is None else (out,)))
-    _heads(q, "q"), _cache(k_cache, "k_cache"), _cache(v_cache, "v_cache", k_cache)
-    (T, hq, d), (pages, hkv, page, dk) = q.shape, k_cache.shape
-    _table(table, page)
-    b, cols = table.shape
-    _i32(kv_lens, "kv_lens", b), _i32(cu_q, "cu_q", b + 1)
-    if d != dk or d not in (64, 128) or q.dtype != k_cache.dtype or hq % hkv or hq < hkv:
-        raise ValueError(f"heads of 64 or 128, a multiple of the cache's heads, in the cache's type: got q {q.dtype} {tuple(q.shape)}, cache {k_cache.dtype} {tuple(k_cache.shape)}")
-    if max_q < 0 or window < 0 or sinks < 0 or (sinks and not window):
-        raise ValueError("max_q, window and sinks are not negative, sinks come with a window")
-    with guard:
-        if out is None:
-            out = q.new_empty((T, hq, d))
-        else:
-            _heads(out, "out")
-            if out.shape != q.shape or out.dtype != q.dtype:
-                raise ValueError("out has the queries' shape and type")
-        L = _lib.lib()
-        need = L.kyb_paged_attention_workspace_bytes(b, T, max_q, cols, page, hq, hkv, d)
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None    # the call's own: captured graphs that replay side by side share nothing
-        qs, os_, ks, vs = q.stride(), out.stride(), k_cache.stride(), v_cache.stride()
-        rc = L.kyb_paged_attention(q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), ks[0], ks[1], v_cache.data_ptr(), vs[0], vs[1], pages, page, table.data_ptr(),
-                                   max(table.stride(0), cols), cols, kv_lens.data_ptr(), cu_q.data_ptr(), b, T, max_q, hq, hkv, d, _DT[q.dtype], d ** -0.5 if scale is None else scale,
-                                   window, sinks, out.data_ptr(), os_[0], os_[1], None if ws is None else ws.data_ptr(), need, _stream())
-        if rc:
-            _lib.check(rc)
+    dev = q.get_device()
+    key = (dev, q.shape, q.stride(), q.dtype, k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape, v_cache.stride(), v_cache.dtype, table.shape, table.stride(), table.dtype, kv_lens.shape,
+           kv_lens.dtype, kv_lens.is_contiguous(), cu_q.shape, cu_q.dtype, cu_q.is_contiguous(), max_q, window, sinks, k_cache.get_device(), v_cache.get_device(), table.get_device(),
+           kv_lens.get_device(), cu_q.get_device(), None if out is None else (out.shape, out.stride(), out.dtype, out.get_device()))
+    known = None if q.requires_grad else _passed.get(key)
+    if known is None:
+        known = _attention_check(key, q, k_cache, v_cache, table, kv_lens, cu_q, max_q, window, sinks, out)
+    if dev != torch.cuda.current_device() if _cur_device is None else dev != _cur_device():
+        with torch.cuda.device(dev):
+            return paged_attention(q, k_cache, v_cache, table, kv_lens, cu_q, max_q, scale, window, sinks, out)
+    need, sizes = known
+    if out is None:
+        out = q.new_empty(q.shape)
+    ws = q.new_empty((need + 1) // 2)                                        # the call's own: captured graphs that replay side by side share nothing
+    rc = _lib.lib().kyb_paged_attention(_lib.PAGED_ATTENTION_ARGS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), kv_lens.data_ptr(), cu_q.data_ptr(), out.data_ptr(),
+                                                                       ws.data_ptr(), *sizes, q.shape[2] ** -0.5 if scale is None else scale), _stream())
+    if rc:
+        _lib.check(rc)
     return out

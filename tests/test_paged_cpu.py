@@ -1,5 +1,7 @@
 """Refusals of the paged-cache operators and their host arithmetic (no GPU needed)."""
 import math
+import os
+import re
 
 import pytest
 import torch
@@ -27,35 +29,48 @@ def test_operators_take_cuda_tensors_only():
 P = 64                       # stands for an address that is 16-byte aligned; every call below is refused before anything is read
 
 
+def _call(entry, block, good, **other):
+    return entry(block.pack(*{**good, **other}.values()), None)
+
+
 def test_step_refusals(lib):
-    good = dict(lens=P, new=P, free=P, cap=10, count=P, table=P, ld=4, batch=2, cols=4, page=16, rows=5)
-    call = lambda **k: lib.kyb_paged_step(*{**good, **k}.values(), P, P, P, P, P, P, P, None)
-    for bad in (dict(lens=None), dict(table=None), dict(cap=0), dict(ld=3), dict(batch=0), dict(batch=1 << 24), dict(cols=0), dict(page=0), dict(page=24), dict(page=8), dict(page=512),
-                dict(rows=-1), dict(rows=1 << 31)):
-        assert call(**bad) == _lib.EINVAL, bad
+    good = dict(lens=P, new=P, free=P, count=P, table=P, cu=P, kv=P, pos=P, slots=P, lens_out=P, count_out=P, refused=P, cap=10, ld=4, batch=2, cols=4, page=16, rows=5)
+    for bad in (dict(lens=0), dict(table=0), dict(slots=0), dict(cap=0), dict(cap=1 << 31), dict(ld=3), dict(batch=0), dict(batch=1 << 24), dict(cols=0), dict(page=0), dict(page=24), dict(page=8),
+                dict(page=512), dict(page=16 + (1 << 32)), dict(page=-16), dict(rows=-1), dict(rows=1 << 31)):
+        assert _call(lib.kyb_paged_step, _lib.PAGED_STEP_ARGS, good, **bad) == _lib.EINVAL, bad
+    assert lib.kyb_paged_step(None, None) == _lib.EINVAL
     assert lib.kyb_paged_release(P, None, P, 4, 2, 4, 16, P, 10, P, P, None) == _lib.EINVAL
     assert lib.kyb_paged_release(P, P, P, 4, 2, 4, 20, P, 10, P, P, None) == _lib.EINVAL
 
 
 def test_rope_refusals(lib):
-    good = dict(q=P, q_t=128, q_h=64, k=P, k_t=64, k_h=64, v=P, v_t=64, v_h=64, pos=P, slots=P, inv=P, tokens=3, hq=2, hkv=1, d=64, rot=64, inter=0, m=1.0, dt=1, qo=P, qo_t=128, qo_h=64,
-                kc=P, kc_p=1024, kc_h=1024, vc=P, vc_p=1024, vc_h=1024, pages=2, page=16)
-    call = lambda **k: lib.kyb_rope_append(*{**good, **k}.values(), None)
-    for bad in (dict(q=None), dict(k=None), dict(slots=None), dict(q=P + 2), dict(vc=P + 8), dict(q_t=100), dict(kc_p=1028), dict(d=60), dict(d=264), dict(rot=0), dict(rot=40), dict(rot=80),
-                dict(dt=0), dict(dt=3), dict(hq=-1), dict(hq=0, hkv=0), dict(tokens=-1), dict(tokens=1 << 31), dict(pages=0), dict(page=48)):
-        assert call(**bad) == _lib.EINVAL, bad
-    assert call(tokens=0) == _lib.OK
+    good = dict(q=P, k=P, v=P, pos=P, slots=P, inv=P, qo=P, kc=P, vc=P, q_t=128, q_h=64, k_t=64, k_h=64, v_t=64, v_h=64, qo_t=128, qo_h=64, kc_p=1024, kc_h=1024, vc_p=1024, vc_h=1024, tokens=3,
+                hq=2, hkv=1, d=64, rot=64, inter=0, dt=1, pages=2, page=16, m=1.0)
+    for bad in (dict(q=0), dict(k=0), dict(slots=0), dict(q=P + 2), dict(vc=P + 8), dict(q_t=100), dict(kc_p=1028), dict(d=60), dict(d=264), dict(rot=0), dict(rot=40), dict(rot=80), dict(dt=0),
+                dict(dt=3), dict(hq=-1), dict(hq=1 << 32), dict(hq=0, hkv=0), dict(tokens=-1), dict(tokens=1 << 31), dict(pages=0), dict(page=48)):
+        assert _call(lib.kyb_rope_append, _lib.ROPE_APPEND_ARGS, good, **bad) == _lib.EINVAL, bad
+    assert _call(lib.kyb_rope_append, _lib.ROPE_APPEND_ARGS, good, tokens=0) == _lib.OK and lib.kyb_rope_append(None, None) == _lib.EINVAL
 
 
 def test_attention_refusals(lib):
-    good = dict(q=P, q_t=128, q_h=64, k=P, k_p=1024, k_h=1024, v=P, v_p=1024, v_h=1024, pages=2, page=16, table=P, ld=3, cols=3, kv=P, cu=P, batch=1, tokens=3, max_q=3, hq=2, hkv=1, d=64,
-                dt=1, scale=0.1, window=0, sinks=0, out=P, o_t=128, o_h=64, ws=P, wsn=1 << 30)
-    call = lambda **k: lib.kyb_paged_attention(*{**good, **k}.values(), None)
-    for bad in (dict(q=None), dict(v=None), dict(table=None), dict(out=None), dict(q=P + 2), dict(out=P + 4), dict(q_t=100), dict(k_p=1028), dict(o_h=-64), dict(pages=0), dict(pages=1 << 31),
-                dict(page=8), dict(page=100), dict(ld=2), dict(cols=0), dict(cols=1 << 28, ld=1 << 28), dict(batch=0), dict(tokens=-1), dict(tokens=1 << 30), dict(max_q=-1), dict(hq=0),
-                dict(hq=3, hkv=2), dict(hq=129), dict(d=96), dict(dt=0), dict(scale=math.nan), dict(scale=math.inf), dict(window=-1), dict(sinks=-1), dict(sinks=4)):
-        assert call(**bad) == _lib.EINVAL, bad
-    assert call(tokens=0) == _lib.OK
+    good = dict(q=P, k=P, v=P, table=P, kv=P, cu=P, out=P, ws=P, q_t=128, q_h=64, k_p=1024, k_h=1024, v_p=1024, v_h=1024, o_t=128, o_h=64, pages=2, page=16, ld=3, cols=3, batch=1, tokens=3,
+                max_q=3, hq=2, hkv=1, d=64, dt=1, window=0, sinks=0, wsn=1 << 30, scale=0.1)
+    for bad in (dict(q=0), dict(v=0), dict(table=0), dict(out=0), dict(q=P + 2), dict(out=P + 4), dict(q_t=100), dict(k_p=1028), dict(o_h=-64), dict(pages=0), dict(pages=1 << 31),
+                dict(page=8), dict(page=100), dict(page=16 + (1 << 32)), dict(ld=2), dict(cols=0), dict(cols=1 << 28, ld=1 << 28), dict(batch=0), dict(tokens=-1), dict(tokens=1 << 30),
+                dict(max_q=-1), dict(max_q=1 << 31), dict(hq=0), dict(hq=3, hkv=2), dict(hq=129), dict(d=96), dict(dt=0), dict(scale=math.nan), dict(scale=math.inf), dict(scale=1e300),
+                dict(window=-1), dict(sinks=-1), dict(sinks=4), dict(tokens=1 << 29, hq=64)):
+        assert _call(lib.kyb_paged_attention, _lib.PAGED_ATTENTION_ARGS, good, **bad) == _lib.EINVAL, bad
+    assert _call(lib.kyb_paged_attention, _lib.PAGED_ATTENTION_ARGS, good, tokens=0) == _lib.OK and lib.kyb_paged_attention(None, None) == _lib.EINVAL
+
+
+def test_argument_blocks_match_the_header():
+    """Sizes of the packed blocks against the structs of include/kyb.h: pointers, int64 and a double, 8 bytes each."""
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "kyb.h")).read()
+    text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
+    for name, block in (("kyb_paged_step_args", _lib.PAGED_STEP_ARGS), ("kyb_rope_append_args", _lib.ROPE_APPEND_ARGS), ("kyb_paged_attention_args", _lib.PAGED_ATTENTION_ARGS)):
+        body = re.search(r"typedef struct \{([^}]*)\} " + name, text).group(1)
+        kinds = "".join(("Q" if "*" in d else "d" if d.strip().startswith("double") else "q") * (d.count(",") + 1) for d in body.split(";") if d.strip())
+        assert kinds == "".join(c * int(n) for n, c in re.findall(r"(\d+)([Qq])", block.format)) + ("d" if block.format.endswith("d") else ""), name
 
 
 def test_rope_frequencies():
