@@ -285,7 +285,7 @@ typedef struct {
 int kyb_rope_append(const kyb_rope_append_args* args, void* stream);
 /* attention of a step's new tokens over the cache: request r owns the rows [cu_q[r], cu_q[r + 1]) of q and out ([tokens][hq][d]), its last row is its token
  * kv_lens[r] - 1. The token at position p sees key j when j <= p and, with window > 0, j > p - window or j < sinks. A row that sees nothing gives zeros; rows outside
- * [cu_q[0], cu_q[batch]) stay as they are. max_q: the largest number of rows of a request (it chooses the kernel; rows of longer requests are served too).
+ * [cu_q[0], cu_q[batch]) stay as they are; out may be q. max_q: the largest number of rows of a request (it chooses the kernel; rows of longer requests are served too).
  * Table entries outside [0, pages) read as tokens of zeros; entries and cache places behind a request's last token, and those in front of the window of its first row,
  * may hold anything. Other places must hold finite values. Scores, sums and the output's accumulation in 32 bits; the weights enter the product with V in the
  * inputs' type, as the tensor cores take them. Scratch: kyb_paged_attention_workspace_bytes, private to the call until it has run. */

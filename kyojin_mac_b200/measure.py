@@ -5,6 +5,7 @@
     python -m kyojin_mac_b200.measure cfg3            # NVFP4 prefill GEMM, 4096 x 7168 -> 18432, activations quantised on the fly
     python -m kyojin_mac_b200.measure fp4peak         # the vendor library's block-scaled NVFP4 GEMM (torch._scaled_mm), a measured fp4 denominator
     python -m kyojin_mac_b200.measure cfg4 [E [T ...]]  # routed-expert layer, E (default 256) experts, top-8, hidden 7168, T = 64 and 4096 (or the given token counts)
+    python -m kyojin_mac_b200.measure attn [B [CTX [NEW]]]  # attention half of the benchmark's layer (hidden 5120, 64 / 8 heads of 128, Q4_K): B requests of CTX cached tokens, NEW each
     python -m kyojin_mac_b200.measure gemv q4_k 27648 5120 1   # one decode product a few times (the target of profiler captures)
     python -m torch.distributed.run --nnodes=1 --nproc-per-node N --master-addr 127.0.0.1 --master-port 29511 -m kyojin_mac_b200.measure dist
                                                       # cfg 2 / 3 N-sharded with all-gather, cfg 4 expert-parallel with all-to-all, on N GPUs
@@ -334,6 +335,35 @@ def router(T=4096, E=256, H=7168, iters=10):
                       "rel_fro_tensor_core": err(ops.router_logits(x, gw, sgw, tensor_cores=True))}), flush=True)
 
 
+def attn_case(batch=64, ctx=4096, new=1, hidden=5120, heads=64, kv_heads=8, d=128, page=64):
+    """The attention half of the benchmark's layer for `batch` requests: slots of the step, q | k | v product, rotary append, attention over ctx cached tokens, o product, as one
+    CUDA graph; the attention call alone beside it."""
+    from .foreign_linear import ForeignLinear
+    from .paged import AttentionBlock, PagedCache
+    n_qkv = (heads + 2 * kv_heads) * d
+    lin = lambda n, k, seed: ForeignLinear(DevPack.from_t16("q4_k", synth.t16_random_device("q4_k", n, k, seed=seed), n, k))
+    block = AttentionBlock(lin(n_qkv, hidden, 1), lin(hidden, heads * d, 2), heads, kv_heads, d, base=500000.0)
+    per = -(-(ctx + new) // page)
+    cache = PagedCache(1, batch * per, kv_heads, d, batch, per * page, page)
+    cache.keys[0].normal_(), cache.values[0].normal_()
+    count, lens = torch.full((batch,), ctx, dtype=torch.int32, device="cuda"), torch.full((batch,), new, dtype=torch.int32, device="cuda")
+    x = torch.randn((batch * new, hidden), device="cuda").to(torch.float16)
+    cache.step(count, 0 if ctx == 0 else batch * ctx)
+
+    def half():                                                               # from the same state each time
+        s = ops.paged_step(cache.table, cache.lens, lens, cache.free_pages, cache.free_count, page, batch * new)
+        return block(x, cache, s, new), s
+    _, s = half()
+    g = graph_of(half)
+    whole = timeit(g.replay)
+    q = torch.randn((batch * new, heads, d), device="cuda").to(torch.float16)
+    ga = graph_of(lambda: ops.paged_attention(q, cache.keys[0], cache.values[0], cache.table, s.kv_lens, s.cu_q, new))
+    att = timeit(ga.replay)
+    keys = batch * (ctx + new)
+    nbytes, flops = 4 * keys * kv_heads * d + 4 * batch * new * heads * d, 4 * heads * d * batch * (new * ctx + new * (new + 1) // 2)
+    return dict(case=f"attn B={batch} ctx={ctx} new={new}", us=whole[0], us_median=whole[1], attention_us=att[0], attention_GBs=nbytes / att[0] / 1e3, attention_TFLOPs=flops / att[0] / 1e6)
+
+
 def main(argv):
     what = argv[0] if argv else "cfg0"
     say = lambda recs: [print(json.dumps(r), flush=True) for r in (recs if isinstance(recs, list) else [recs])]
@@ -370,6 +400,8 @@ def main(argv):
         for _ in range(3):
             y = dp.apply_a4(x)
         print(json.dumps({"case": f"gemm_a4 nvfp4 {n}x{k} m={m}", "mean_abs": float(y.float().abs().mean())}), flush=True)
+    elif what == "attn":
+        print(json.dumps(attn_case(*(int(a) for a in argv[1:4]))), flush=True)
     elif what == "dist":
         dist_cases(int(argv[1]) if len(argv) > 1 else 256)
     else:

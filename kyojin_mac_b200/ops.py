@@ -743,7 +743,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     """Attention of a step's new tokens over a paged cache: q fp16 / bf16 [T, heads, d] packed by request (rows [cu_q[r], cu_q[r + 1]); the last one is token
     kv_lens[r] - 1), keys and values through the block table [batch, columns]. Causal; window > 0: the last `window` tokens only, and the first `sinks` ones.
     max_q: the largest number of new tokens of a request (chooses the kernel; requests with more are served all the same). scale: d ** -0.5 unless given.
-    A row that sees nothing (kv_lens 0) gives zeros; rows behind the last request are left as they were (undefined without `out`). Returns out [T, heads, d]."""
+    A row that sees nothing (kv_lens 0) gives zeros; rows behind the last request are left as they were (undefined without `out`). `out` may be q itself. Returns out [T, heads, d]."""
     dev = q.get_device()
     key = (dev, q.shape, q.stride(), q.dtype, k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape, v_cache.stride(), v_cache.dtype, table.shape, table.stride(), table.dtype, kv_lens.shape,
            kv_lens.dtype, kv_lens.is_contiguous(), cu_q.shape, cu_q.dtype, cu_q.is_contiguous(), max_q, window, sinks, k_cache.get_device(), v_cache.get_device(), table.get_device(),
