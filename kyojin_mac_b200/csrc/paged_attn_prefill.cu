@@ -7,8 +7,8 @@
 //   10         clears values in places that no row sees (11 is idle: registers move between groups of four warps, from these four to the softmax)
 // Tensor memory: S0 | S1 | O0 | O1, 128 columns each; the weights P (16 bits) take the place of their scores S. S = Q K^T with both operands in shared memory; O += P V with
 // P in tensor memory and V as it lies in the cache (MN-major operand). The issuer's order S0(j+1) behind O0(j), S1(j+1) behind O1(j) keeps the tensor cores busy
-// with one query tile while the softmax of the other runs. A row's reference maximum moves only when a score passes it by 2^8, so O is rescaled (by the softmax warps
-// themselves, in tensor memory) a few times per row at most; sums are of the unrounded weights, in 32 bits.
+// with one query tile while the softmax of the other runs. A row's reference maximum moves only when a score passes it by 2^15, so O is rescaled (by the softmax warps
+// themselves, in tensor memory) hardly ever; sums are of the unrounded weights, in 32 bits.
 // Keys that a row does not see are masked by selection in the tiles at the borders; values in places that no row of the block sees are cleared in shared memory, since such
 // places may hold anything and 0 times NaN is NaN.
 #include <algorithm>
@@ -441,21 +441,51 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_attn_prefill_kernel(const
                                 if (!(see >> e & 1u)) v[q][e] = 0xff800000u;
                         }
                     }
+                    // weights of 32 keys to tensor memory, their sum added to `sum`
+                    uint64_t m_pair, sum[2];
+                    auto reference = [&]() {
+                        const float m0 = m == -INFINITY ? 0.f : -m;
+                        m_pair = pair_of(m0, m0), sum[0] = sum[1] = 0;
+                    };
                     float t[4];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        float a = max3(__uint_as_float(v[q][0]), __uint_as_float(v[q][1]), __uint_as_float(v[q][2]));
+                    for (int q = 0; q < 4; ++q) t[q] = fmaxf(__uint_as_float(v[q][0]), __uint_as_float(v[q][1]));
+                    auto weights = [&](int q, bool find_top) {
+                        uint32_t pk[16];
 #pragma unroll
-                        for (int e = 3; e < 31; e += 2) a = max3(a, __uint_as_float(v[q][e]), __uint_as_float(v[q][e + 1]));
-                        t[q] = fmaxf(a, __uint_as_float(v[q][31]));
+                        for (int e = 0; e < 32; e += 2) {
+                            float a, b;
+                            split_pair(fma_pair(pair_of(__uint_as_float(v[q][e]), __uint_as_float(v[q][e + 1])), scale_pair, m_pair), a, b);
+                            a = exp2_fast(a), b = exp2_fast(b);
+                            sum[(e >> 1) & 1] = add_pair(sum[(e >> 1) & 1], pair_of(a, b));
+                            pk[e / 2] = pack2<T>(a, b);
+                            if (find_top && e) {
+                                t[q] = max3(t[q], __uint_as_float(v[q][e]), __uint_as_float(v[q][e + 1]));
+                                t[q + 2 & 3] = max3(t[q + 2 & 3], __uint_as_float(v[q + 2 & 3][e]), __uint_as_float(v[q + 2 & 3][e + 1]));
+                            }
+                        }
+                        tmem_st_16(ts + 16 * q, pk);
+                    };
+                    // With heads of 64 the first half's weights are made with the reference as it is while the maximum is found, and again in the rare tile where a score
+                    // passes the reference by 2^15, beyond which fp16 would overflow: 219 -> 208 us for 1024 tokens on 8192. With heads of 128, where the wait for the
+                    // products is the longer part, it gained nothing (252 -> 255 us): there, as in the first tile of an item, the maximum comes first.
+                    if (D == 64 && i) {
+                        reference();
+                        weights(0, true), weights(1, true);
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+#pragma unroll
+                            for (int e = 2; e < 32; e += 2) t[q] = max3(t[q], __uint_as_float(v[q][e]), __uint_as_float(v[q][e + 1]));
                     }
                     const float top = fmaxf(max3(t[0], t[1], t[2]), t[3]) * scale2;
-                    const bool over = top > m + 8.f;                         // false where nothing is seen yet (-inf on both sides)
-                    if (__any_sync(0xffffffffu, over)) {
+                    const bool over = top > m + 15.f;                        // false where nothing is seen yet (-inf on both sides)
+                    const bool move = __any_sync(0xffffffffu, over);
+                    if (move || D != 64 || i == 0) {
                         const float f = !over ? 1.f : m == -INFINITY ? 0.f : exp2_fast(m - top);
                         if (over) m = top;
                         l *= f;
-                        if (i) {
+                        if (i && (D == 64 || move)) {
 #pragma unroll 1
                             for (int q = 0; q < D; q += 16) {
                                 uint32_t x[16];
@@ -466,31 +496,20 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_attn_prefill_kernel(const
                                 tmem_st_16(to + q, x);
                             }
                         }
+                        reference();
+                        weights(0, false), weights(1, false);
                     }
-                    const float m0 = m == -INFINITY ? 0.f : -m;
-                    const uint64_t m_pair = pair_of(m0, m0);
-                    uint64_t sum0 = 0, sum1 = 0;                             // two pairs of zeros
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        uint32_t pk[16];
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
-                            float a, b;
-                            split_pair(fma_pair(pair_of(__uint_as_float(v[q][e]), __uint_as_float(v[q][e + 1])), scale_pair, m_pair), a, b);
-                            a = exp2_fast(a), b = exp2_fast(b);
-                            if (e & 2) sum1 = add_pair(sum1, pair_of(a, b)); else sum0 = add_pair(sum0, pair_of(a, b));
-                            pk[e / 2] = pack2<T>(a, b);
-                        }
-                        tmem_st_16(ts + 16 * q, pk);
-                        if (q & 1) {                                         // the weights of 64 keys are there
-                            tmem_st_wait_all();
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive_a(q == 1 ? pfull : phalf);
-                        }
-                    }
+                    auto hand_over = [&](uint32_t bar) {
+                        tmem_st_wait_all();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_a(bar);
+                    };
+                    hand_over(pfull);
+                    weights(2, false), weights(3, false);
+                    hand_over(phalf);
                     float a, b;
-                    split_pair(add_pair(sum0, sum1), a, b);
+                    split_pair(add_pair(sum[0], sum[1]), a, b);
                     l += a + b;
                 }
                 if (!failed && !wait_here(sfull, sparity)) failed = true;    // the last O
