@@ -273,7 +273,7 @@ int kyb_paged_release(void* lens, const void* which, void* table, int64_t ld_tab
 /* rotary positions and cache append: the pairs of the first rot values of every query and key head (interleaved: (2 i, 2 i + 1), else (i, i + rot / 2)) turned by
  * positions[t] * inv_freq[i] (fp32 [rot / 2]; product and reduction in 64 bits) and scaled by mscale; queries to q_out (may be q), keys and values to the cache at
  * slots[t]. A row with positions[t] < 0 is left alone, a slot outside the cache stores nothing. hkv = 0: queries only. d a multiple of 8 up to 256, rot a
- * multiple of 16. Strides in elements. Slots that two rows share hold one of them in the end. */
+ * multiple of 16. Strides in elements. A slot that two rows share holds values of either. */
 typedef struct {
     const void *q, *k, *v, *positions, *slots, *inv_freq;
     void *q_out, *k_cache, *v_cache;

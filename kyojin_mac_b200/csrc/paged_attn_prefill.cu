@@ -20,8 +20,9 @@ namespace kyb {
 
 constexpr int PF_TILE = 128, PF_THREADS = 384;
 
-// An item costs about three tiles beyond its own (query load, the first scores, the last values, the output): measured.
-using PrefillRuns = Runs<3, 1>;
+// An item costs about two tiles beyond its own (query load, the first scores, the last values, the output). Measured over nine shapes from 20 to 4001 new tokens: two and a
+// snap of one on average 1 % faster than three, with eight prompts of 2048 tokens take 96 instead of 85 us.
+using PrefillRuns = Runs<2, 1>;
 
 template <int D>
 struct PrefillShape {
@@ -139,8 +140,9 @@ __device__ __forceinline__ void find_run_wide(const AttnParams& p, int block, Ru
     }
     const int ctas = min((int)gridDim.x, total), c = blockIdx.x;
     const int u0 = c < ctas ? run_border(total, ctas, c) : 0, u1 = c < ctas ? run_border(total, ctas, c + 1) : 0;
-    if (tid == 0) f.run.left = 0;
+    if (tid == 0) f.run.left = 0, f.request = 0, f.at = 0;
     if (u1 == u0) return;
+    __syncthreads();
     int before = 0;
     for (int r0 = 0; r0 < p.batch && before <= u0; r0 += PF_THREADS) {
         if (p.batch > PF_THREADS) {

@@ -532,6 +532,13 @@ def _heads(t, name):
         raise ValueError(f"{name}: heads must be dense, strides multiples of 8 elements, the start 16-byte aligned; got strides {t.stride()}")
 
 
+def _own_rows(t, name):
+    """An output [tokens, heads, d] whose heads do not overlap in memory."""
+    (n0, s0), (n1, s1) = sorted(((t.shape[0], t.stride(0)), (t.shape[1], t.stride(1))), key=lambda p: p[1])
+    if t.numel() and ((n0 > 1 and s0 < t.shape[2]) or (n1 > 1 and s1 < (s0 * n0 if n0 > 1 else t.shape[2]))):
+        raise ValueError(f"{name}: heads overlap in memory, strides {t.stride()}")
+
+
 def _cache(t, name, like=None):
     if t.dtype not in (torch.float16, torch.bfloat16) or t.dim() != 4 or t.shape[2] not in (16, 32, 64, 128, 256) or (like is not None and (t.shape != like.shape or t.dtype != like.dtype)):
         raise ValueError(f"{name} must be float16 or bfloat16 [pages, kv heads, 16 .. 256 (a power of two), d], keys and values alike, got {t.dtype} {tuple(t.shape)}")
@@ -656,7 +663,7 @@ def _rope_check(key, q, k, v, positions, slots, inv_freq, kc, vc, out):
         raise ValueError("inv_freq is contiguous float32 [rot / 2]")
     T, hq, d = q.shape
     if out is not None:
-        _heads(out, "out")
+        _heads(out, "out"), _own_rows(out, "out")
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError("out has the queries' shape and type")
     ks = vs = kcs = vcs = (0, 0)
@@ -704,7 +711,7 @@ def _rope_call(q, k, v, positions, slots, inv_freq, kc, vc, interleaved, mscale,
 
 def rope(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False, mscale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
     """x fp16 / bf16 [tokens, heads, d] with the first rot = 2 len(inv_freq) values of every head turned: pairs (i, i + rot / 2), or (2 i, 2 i + 1) when interleaved, by
-    positions[t] * inv_freq[i], scaled by mscale. Rows of a negative position are left as they are in `out` (which may be x)."""
+    positions[t] * inv_freq[i], scaled by mscale. Rows of a negative position are left as they are in `out` (which may be x, or memory apart from it)."""
     return _rope_call(x, None, None, positions, None, inv_freq, None, None, interleaved, mscale, out)
 
 
@@ -712,7 +719,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
                 interleaved: bool = False, mscale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
     """`rope` of a step's queries, and in the same launch its keys (turned) and values into the cache [pages, kv heads, tokens of a page, d] at slots[t]. q [T, heads, d],
     k and v [T, kv heads, d] may be views of one q | k | v product. Returns the turned queries. Rows with a negative position are left alone, a slot outside the cache
-    stores nothing; of rows that share a slot one is stored."""
+    stores nothing. The slots of a step are distinct (paged_step's are): one that two rows share holds values of either."""
     return _rope_call(q, k, v, positions, slots, inv_freq, k_cache, v_cache, interleaved, mscale, out)
 
 
@@ -728,7 +735,7 @@ def _attention_check(key, q, kc, vc, table, kv_lens, cu_q, max_q, window, sinks,
     if max_q < 0 or window < 0 or sinks < 0 or (sinks and not window):
         raise ValueError("max_q, window and sinks are not negative, sinks come with a window")
     if out is not None:
-        _heads(out, "out")
+        _heads(out, "out"), _own_rows(out, "out")
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError("out has the queries' shape and type")
     with torch.cuda.device(q.device):

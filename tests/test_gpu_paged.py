@@ -348,3 +348,102 @@ def test_steps_in_a_row():
             assert ((out[at].cpu().double() - want).abs() <= tol + more).all(), (new, r)
     assert ops.paged_release(table, lens, torch.tensor([True, False, True], device="cuda"), free, count, page).item() == 0
     assert lens.tolist()[0] == 0 and count.item() == 40 - (-(-int(lens[1]) // page))
+
+
+# ------------------------------------------------------------------------------------------------ layouts, large offsets, calls out of the ordinary
+@pytest.mark.parametrize("qn", [[1, 2, 1], [60, 1, 33]])
+def test_heads_apart_and_transposed(qn):
+    """Queries and output whose heads are not neighbours: every second block of d values; heads outside, tokens inside; keys head by head over all pages."""
+    kv, hq, hkv, d, page = [70, 200, 33], 8, 2, 128, 16
+    k, v, table = R.pool(kv, page, hkv, d, F16, 21)
+    t = sum(qn)
+    q = torch.randn((t, hq, d), device="cuda").to(F16)
+    lens, cu = _i32(kv), _i32([sum(qn[:i]) for i in range(4)])
+    want = ops.paged_attention(q, k, v, table, lens, cu, max(qn))
+    for lay in ("apart", "heads first"):
+        mk = (lambda: torch.zeros((t, hq, 2, d), dtype=F16, device="cuda")[:, :, 1]) if lay == "apart" else (lambda: torch.zeros((hq, t, d), dtype=F16, device="cuda").transpose(0, 1))
+        q2, out = mk(), mk()
+        q2.copy_(q)
+        assert torch.equal(ops.paged_attention(q2, k, v, table, lens, cu, max(qn), out=out), want)
+        inv, _ = ops.rope_frequencies(d)
+        pos = torch.arange(t, device="cuda").to(torch.int32)
+        assert torch.equal(ops.rope(q2, pos, inv, out=mk()), ops.rope(q, pos, inv))
+    k2, v2 = (x.transpose(0, 1).contiguous().transpose(0, 1) for x in (k, v))        # [head][page] in memory
+    assert torch.equal(ops.paged_attention(q, k2, v2, table, lens, cu, max(qn)), want)
+    for bad in (q[:1].expand(t, hq, d), q[:, :1].expand(t, hq, d)):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.paged_attention(q, k, v, table, lens, cu, max(qn), out=bad)
+
+
+@pytest.mark.parametrize("qn", [[1, 2, 1], [60, 1, 133], [7, 300, 4]])
+def test_output_in_the_queries_place(qn):
+    kv = [70, 900, 333]
+    k, v, table = R.pool(kv, 32, 2, 128, BF16, 22)
+    q = torch.randn((sum(qn) + 2, 8, 128), device="cuda").to(BF16)
+    lens, cu = _i32(kv), _i32([sum(qn[:i]) for i in range(4)])
+    want = ops.paged_attention(q, k, v, table, lens, cu, max(qn), out=q.clone())
+    assert ops.paged_attention(q, k, v, table, lens, cu, max(qn), out=q) is q and torch.equal(q, want)
+
+
+def test_cache_beyond_four_gigabytes():
+    """Pages whose bytes lie behind 2^32 (and values behind 2^31): append and attention reach them."""
+    page, hkv, d, n = 64, 8, 128, 40000                                      # 5.2 GB each
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("16 GB of free device memory needed")
+    kc, vc = (torch.empty((n, hkv, page, d), dtype=F16, device="cuda") for _ in range(2))
+    t, ids = 150, [n - 1, 5, n - 7]
+    g = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn((t, h, d), generator=g).to(F16).cuda() for h in (16, hkv, hkv))
+    pos = torch.arange(t)
+    slots = torch.tensor([ids[p // page] * page + p % page for p in range(t)], dtype=torch.int32).cuda()
+    inv, _ = ops.rope_frequencies(d)
+    qt = ops.rope_append(q, k, v, pos.to(torch.int32).cuda(), slots, inv, kc, vc)
+    table, small = _i32([ids]), _i32([[0, 1, 2]])
+    ks, vs = (c[torch.tensor(ids, device="cuda")].clone() for c in (kc, vc))
+    for lens, cu in ((_i32([t]), _i32([0, t])), (_i32([t]), _i32([0, 1]))):
+        rows = int(cu[1])
+        got = ops.paged_attention(qt[:rows], kc, vc, table, lens, cu, rows)
+        assert torch.equal(got, ops.paged_attention(qt[:rows], ks, vs, small, lens, cu, rows))
+        want, tol = R.attention(qt[:rows], ks, vs, small, lens, cu, d ** -0.5, 0, 0)
+        assert ((got.cpu().double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("qn", [1, 40])
+def test_row_offsets_out_of_order(qn):
+    """Offsets that fall, are negative or lie behind the rows reach no memory outside the tensors: the kernels bring them inside. Requests with good ones are served."""
+    kv = [50, 60, 70]
+    k, v, table = R.pool(kv, 16, 1, 64, F16, 23)
+    whole = torch.zeros((3 * qn + 6, 8, 64), dtype=F16, device="cuda")
+    q = whole[3:3 * qn + 3]
+    q.normal_()
+    good = [0, qn, 2 * qn, 3 * qn]
+    want = ops.paged_attention(q, k, v, table, _i32(kv), _i32(good), qn)
+    for cu in ([0, qn, -5, -9], [0, qn, 10 ** 9, 2 ** 31 - 1], [0, qn, qn, -2 ** 31]):
+        out = torch.zeros_like(whole)
+        ops.paged_attention(q, k, v, table, _i32(kv), _i32(cu), qn, out=out[3:3 * qn + 3])
+        assert torch.equal(out[3:3 + qn], want[:qn]) and (out[:3] == 0).all() and (out[3 * qn + 3:] == 0).all()
+    out = ops.paged_attention(q, k, v, table, _i32([-4, 50 * 2 ** 20, 70]), _i32(good), qn)      # lengths that are negative or beyond any table
+    assert (out[:qn] == 0).all() and torch.equal(out[2 * qn:], want[2 * qn:])
+    ops.check_device_status()
+
+
+def test_another_stream_and_threads():
+    """Calls on side streams, from two host threads at once, give what calls in a row give."""
+    import threading
+    k, v, table = R.pool([700, 300], 32, 2, 128, F16, 24)
+    lens = _i32([700, 300])
+    jobs = [(torch.randn((n * 2, 8, 128), device="cuda").to(F16), _i32([0, n, 2 * n]), n) for n in (1, 30, 2, 90)]
+    want = [ops.paged_attention(q, k, v, table, lens, cu, n) for q, cu, n in jobs]
+    torch.cuda.synchronize()
+    got = [[None] * 4 for _ in range(2)]
+
+    def work(who):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                for i, (q, cu, n) in enumerate(jobs):
+                    got[who][i] = ops.paged_attention(q, k, v, table, lens, cu, n)
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(w,)) for w in range(2)]
+    [t.start() for t in threads], [t.join() for t in threads]
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+
