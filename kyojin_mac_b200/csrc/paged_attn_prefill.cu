@@ -9,6 +9,8 @@
 // P in tensor memory and V as it lies in the cache (MN-major operand). The issuer's order S0(j+1) behind O0(j), S1(j+1) behind O1(j) keeps the tensor cores busy
 // with one query tile while the softmax of the other runs. A row's reference maximum moves only when a score passes it by 2^15, so O is rescaled (by the softmax warps
 // themselves, in tensor memory) hardly ever; sums are of the unrounded weights, in 32 bits.
+// Measured, 64 / 8 heads of 128: 1024 tokens on 8192 cached ones 245 to 250 us, a prompt of 8192 tokens 910 us = 1210 TFLOP/s; 3200 clocks a pair of tiles, of which the tensor
+// cores and the special-function units are busy 2050 each.
 // Keys that a row does not see are masked by selection in the tiles at the borders; values in places that no row of the block sees are cleared in shared memory, since such
 // places may hold anything and 0 times NaN is NaN.
 #include <algorithm>

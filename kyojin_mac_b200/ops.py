@@ -16,6 +16,9 @@ from .layout import FMT_ID, padded_rows
 _raw_stream, _cur_device = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None)
 
 
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+
+
 def _stream() -> int:
     if _raw_stream is None or not torch.cuda.is_initialized():
         return torch.cuda.current_stream().cuda_stream
@@ -577,8 +580,9 @@ def paged_step(table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor, 
     A request is served when its pages fit the columns, its tokens the rows, and the needs of the requests up to its own the free list (one that needs no page
     is not held up); `refused` counts the others, whose lengths stay. in_place: lens and free_count are updated too (a captured step that is replayed)."""
     dev = table.get_device()
-    key = (dev, table.shape, table.stride(), table.dtype, lens.shape, lens.dtype, lens.is_contiguous(), new_lens.shape, new_lens.dtype, new_lens.is_contiguous(), free_pages.shape, free_pages.dtype,
-           free_pages.is_contiguous(), free_count.shape, free_count.dtype, page, rows, in_place, lens.get_device(), new_lens.get_device(), free_pages.get_device(), free_count.get_device())
+    key = (dev, table.shape, table.is_contiguous() or table.stride(), table.dtype, lens.shape, lens.dtype, lens.is_contiguous(), new_lens.shape, new_lens.dtype, new_lens.is_contiguous(),
+           free_pages.shape, free_pages.dtype, free_pages.is_contiguous(), free_count.shape, free_count.dtype, page, rows, in_place, lens.get_device(), new_lens.get_device(), free_pages.get_device(),
+           free_count.get_device())
     known = _passed.get(key)
     if known is None:
         _place(table, lens, new_lens, free_pages, free_count)
@@ -588,15 +592,19 @@ def paged_step(table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor, 
         if free_pages.numel() < 1 or rows < 0:
             raise ValueError("the free list is an array with room for a page at least, rows not negative")
         sizes = [b + 1, b, rows, rows, 1] + ([] if in_place else [b, 1])
-        known = _remember(key, (sum(sizes), sizes, (free_pages.shape[0], max(table.stride(0), cols), b, cols, page, rows)))
+        offs = [4 * sum(sizes[:i]) for i in range(len(sizes))]
+        known = _remember(key, (sum(sizes), sizes, offs, (free_pages.shape[0], max(table.stride(0), cols), b, cols, page, rows)))
     if dev != torch.cuda.current_device() if _cur_device is None else dev != _cur_device():
         with torch.cuda.device(dev):
             return paged_step(table, lens, new_lens, free_pages, free_count, page, rows, in_place)
-    total, sizes, numbers = known
-    cu, kv, pos, slots, refused, *more = lens.new_empty(total).split_with_sizes(sizes)
+    total, sizes, offs, numbers = known
+    buf = lens.new_empty(total)                                              # all results side by side
+    at, lens_p, count_p = buf.data_ptr(), lens.data_ptr(), free_count.data_ptr()
+    cu, kv, pos, slots, refused, *more = buf.split_with_sizes(sizes)
     out_lens, out_count = (lens, free_count) if in_place else more
-    rc = _lib.lib().kyb_paged_step(_lib.PAGED_STEP_ARGS.pack(lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), table.data_ptr(), cu.data_ptr(), kv.data_ptr(),
-                                                             pos.data_ptr(), slots.data_ptr(), out_lens.data_ptr(), out_count.data_ptr(), refused.data_ptr(), *numbers), _stream())
+    out_lens_p, out_count_p = (lens_p, count_p) if in_place else (at + offs[5], at + offs[6])
+    rc = _lib.lib().kyb_paged_step(_lib.PAGED_STEP_ARGS.pack(lens_p, new_lens.data_ptr(), free_pages.data_ptr(), count_p, table.data_ptr(), at, at + offs[1], at + offs[2], at + offs[3], out_lens_p,
+                                                             out_count_p, at + offs[4], *numbers), _stream())
     if rc:
         _lib.check(rc)
     return PagedStep(cu, kv, pos, slots, out_lens, out_count, refused)
@@ -686,8 +694,8 @@ def _rope_call(q, k, v, positions, slots, inv_freq, kc, vc, interleaved, mscale,
     else:
         grad = grad or k.requires_grad or v.requires_grad
         key = (dev, q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, positions.shape, positions.dtype, positions.is_contiguous(), slots.shape, slots.dtype,
-               slots.is_contiguous(), inv_freq.shape, inv_freq.dtype, kc.shape, kc.stride(), kc.dtype, vc.shape, vc.stride(), vc.dtype, k.get_device(), v.get_device(), positions.get_device(),
-               slots.get_device(), inv_freq.get_device(), kc.get_device(), vc.get_device())
+               slots.is_contiguous(), inv_freq.shape, inv_freq.dtype, kc.shape, kc.is_contiguous() or kc.stride(), kc.dtype, vc.shape, vc.is_contiguous() or vc.stride(), vc.dtype, k.get_device(),
+               v.get_device(), positions.get_device(), slots.get_device(), inv_freq.get_device(), kc.get_device(), vc.get_device())
     if out is not None:
         key += (out.shape, out.stride(), out.dtype, out.get_device())
     sizes = None if grad or not inv_freq.is_contiguous() else _passed.get(key)
@@ -697,7 +705,7 @@ def _rope_call(q, k, v, positions, slots, inv_freq, kc, vc, interleaved, mscale,
         with torch.cuda.device(dev):
             return _rope_call(q, k, v, positions, slots, inv_freq, kc, vc, interleaved, mscale, out)
     if out is None:
-        out = q.new_empty(q.shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if k is None:
         ptrs, pages = (q.data_ptr(), 0, 0, positions.data_ptr(), 0, inv_freq.data_ptr(), out.data_ptr(), 0, 0), (0, 0)
     else:
@@ -752,9 +760,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     max_q: the largest number of new tokens of a request (chooses the kernel; requests with more are served all the same). scale: d ** -0.5 unless given.
     A row that sees nothing (kv_lens 0) gives zeros; rows behind the last request are left as they were (undefined without `out`). `out` may be q itself. Returns out [T, heads, d]."""
     dev = q.get_device()
-    key = (dev, q.shape, q.stride(), q.dtype, k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape, v_cache.stride(), v_cache.dtype, table.shape, table.stride(), table.dtype, kv_lens.shape,
-           kv_lens.dtype, kv_lens.is_contiguous(), cu_q.shape, cu_q.dtype, cu_q.is_contiguous(), max_q, window, sinks, k_cache.get_device(), v_cache.get_device(), table.get_device(),
-           kv_lens.get_device(), cu_q.get_device(), None if out is None else (out.shape, out.stride(), out.dtype, out.get_device()))
+    key = (dev, q.shape, q.is_contiguous() or q.stride(), q.dtype, k_cache.shape, k_cache.is_contiguous() or k_cache.stride(), k_cache.dtype, v_cache.shape,
+           v_cache.is_contiguous() or v_cache.stride(), v_cache.dtype, table.shape, table.is_contiguous() or table.stride(), table.dtype, kv_lens.shape, kv_lens.dtype, kv_lens.is_contiguous(),
+           cu_q.shape, cu_q.dtype, cu_q.is_contiguous(), max_q, window, sinks, k_cache.get_device(), v_cache.get_device(), table.get_device(), kv_lens.get_device(), cu_q.get_device(),
+           None if out is None else (out.shape, out.stride(), out.dtype, out.get_device()))
     known = None if q.requires_grad else _passed.get(key)
     if known is None:
         known = _attention_check(key, q, k_cache, v_cache, table, kv_lens, cu_q, max_q, window, sinks, out)
@@ -763,8 +772,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             return paged_attention(q, k_cache, v_cache, table, kv_lens, cu_q, max_q, scale, window, sinks, out)
     need, sizes = known
     if out is None:
-        out = q.new_empty(q.shape)
-    ws = q.new_empty((need + 1) // 2)                                        # the call's own: captured graphs that replay side by side share nothing
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    # scratch: the stream's own, or inside a capture the call's, so that captured graphs that replay side by side share nothing
+    ws = q.new_empty((need + 1) // 2) if _capturing() else workspace(q.device, need)
     rc = _lib.lib().kyb_paged_attention(_lib.PAGED_ATTENTION_ARGS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), kv_lens.data_ptr(), cu_q.data_ptr(), out.data_ptr(),
                                                                        ws.data_ptr(), *sizes, q.shape[2] ** -0.5 if scale is None else scale), _stream())
     if rc:
