@@ -352,17 +352,20 @@ __global__ void __launch_bounds__(DC_THREADS, 2) paged_attn_decode_kernel(const 
     if (failed) atomicExch(p.status, KYB_DEV_TIMEOUT_ATTN);
 }
 
-// The parts of the items that begin in run blockIdx.x and end in a later one: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i, in the order of the runs. A warp per
-// row, a lane holds D / 32 of its values; the parts' maxima and sums are read 32 at a time.
-constexpr int JOIN_ROWS = 8;
-template <typename T, int D>
-__global__ void __launch_bounds__(32 * JOIN_ROWS) paged_attn_join_kernel(const AttnParams p, const int ctas, const int block) {
+// The parts of the items that begin in run blockIdx.x and end in a later one: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i, in a fixed order. PER_ROW warps a row,
+// each with every PER_ROW-th part; a lane holds D / 32 of the row's values, the parts' maxima and sums are read 32 at a time. After the decode kernel a row may have a part from
+// each of 296 runs (one long context, one key-value head): a block of four warps per row then, so that several SMs read the parts' megabyte (125 000 keys of one head 44 -> 31 us
+// in all; eight warps 25, but 1 to 2 us more for every call with little to join). After the prefill kernel it has a few, and a block takes eight of up to 256 rows: many blocks
+// that find nothing cost more.
+template <typename T, int D, int JOIN_WARPS, int PER_ROW>
+__global__ void __launch_bounds__(32 * JOIN_WARPS) paged_attn_join_kernel(const AttnParams p, const int ctas, const int block) {
     constexpr int E = D / 32;
+    __shared__ float meet[PER_ROW > 1 ? JOIN_WARPS : 1][D + 1];
     pdl_launch_dependents();
     pdl_wait();
-    const int first = blockIdx.x, lane = threadIdx.x & 31;
+    const int first = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % PER_ROW;
     const int4 note = p.notes[first];
-    const int rr = blockIdx.y * JOIN_ROWS + (threadIdx.x >> 5);
+    const int rr = blockIdx.y * (JOIN_WARPS / PER_ROW) + warp / PER_ROW;
     if (!(note.w & NOTE_BEGINS) || rr >= block) return;
     int row_base;
     const int tokens = request_rows(p, note.x, row_base), row = note.y * block + rr, tok = row / p.group;
@@ -375,24 +378,25 @@ __global__ void __launch_bounds__(32 * JOIN_ROWS) paged_attn_join_kernel(const A
         n += ends ? __ffs(ends) : 32, more = !ends;
     }
     n = min(n, ctas - first);
-    const float* const head = p.parts + ((size_t)first * 2 + 1) * size, * const rest = p.parts + (size_t)(first + 1) * 2 * size;   // part 0, and part i at rest + 2 (i - 1) size
+    auto part = [&](int i) { return p.parts + ((size_t)(first + i) * 2 + (i == 0)) * size; };
     float top = -INFINITY;
-    for (int i = lane; i < n; i += 32) top = fmaxf(top, (i ? rest + (size_t)(i - 1) * 2 * size : head)[(size_t)block * D + rr]);
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, part(i)[(size_t)block * D + rr]);
 #pragma unroll
     for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
     float o[E] = {}, sum = 0.f;
-    for (int i0 = 0; i0 < n; i0 += 32) {
-        const int i = i0 + lane;
+    const int mine = (n - share + PER_ROW - 1) / PER_ROW;                    // parts share, share + PER_ROW, ...
+    for (int i0 = 0; i0 < mine; i0 += 32) {
+        const int i = share + (i0 + lane) * PER_ROW;
         float w = 0.f;
-        if (i < n) {
-            const float* const x = (i ? rest + (size_t)(i - 1) * 2 * size : head) + (size_t)block * D + rr;
+        if (i0 + lane < mine) {
+            const float* const x = part(i) + (size_t)block * D + rr;
             w = x[0] == -INFINITY ? 0.f : exp2f(x[0] - top);
             sum += w * x[block];
         }
-        const int k = min(32, n - i0);
+        const int k = min(32, mine - i0);
 #pragma unroll 4
         for (int j = 0; j < k; ++j) {
-            const float* const x = (i0 + j ? rest + (size_t)(i0 + j - 1) * 2 * size : head) + (size_t)rr * D + lane * E;
+            const float* const x = part(share + (i0 + j) * PER_ROW) + (size_t)rr * D + lane * E;
             const float wj = __shfl_sync(0xffffffffu, w, j);
             if constexpr (E == 4) {
                 const float4 v = *reinterpret_cast<const float4*>(x);
@@ -405,6 +409,18 @@ __global__ void __launch_bounds__(32 * JOIN_ROWS) paged_attn_join_kernel(const A
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if constexpr (PER_ROW > 1) {                                             // (all warps of a row's block come here or none)
+#pragma unroll
+        for (int e = 0; e < E; ++e) meet[warp][lane * E + e] = o[e];
+        if (lane == 0) meet[warp][D] = sum;
+        __syncthreads();
+        if (share) return;
+        for (int w = 1; w < PER_ROW; ++w) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += meet[warp + w][lane * E + e];
+            sum += meet[warp + w][D];
+        }
+    }
     const float inv = sum > 0.f ? 1.f / sum : 0.f;
     T* const out = reinterpret_cast<T*>(p.o) + (int64_t)(row_base + tok) * p.o_t + (int64_t)(note.z * p.group + row - tok * p.group) * p.o_h + lane * E;
 #pragma unroll
@@ -449,19 +465,21 @@ int kyb_attn_decode(KybAttnCall& c, int rows, void* ws) {
     return wide ? launch_decode<__nv_bfloat16, 128, 2>(c, ws) : launch_decode<__nv_bfloat16, 128, 1>(c, ws);
 }
 
-int kyb_attn_join(const KybAttnCall& c, int ctas, int block) {
+template <typename T, int D>
+static int launch_join(const KybAttnCall& c, int ctas, int block) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ctas, (unsigned)((block + kyb::JOIN_ROWS - 1) / kyb::JOIN_ROWS)), cfg.blockDim = dim3(32 * kyb::JOIN_ROWS), cfg.stream = c.st;
+    const bool few = block <= KYB_DECODE_ROWS;
+    cfg.gridDim = dim3((unsigned)ctas, (unsigned)(few ? block : (block + 7) / 8)), cfg.blockDim = dim3(few ? 128 : 256), cfg.stream = c.st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at, cfg.numAttrs = 1;
-    if (c.dtype == 1) {
-        if (c.d == 64) KYB_CUDA(cudaLaunchKernelEx(&cfg, kyb::paged_attn_join_kernel<__half, 64>, c.p, ctas, block));
-        else KYB_CUDA(cudaLaunchKernelEx(&cfg, kyb::paged_attn_join_kernel<__half, 128>, c.p, ctas, block));
-    } else {
-        if (c.d == 64) KYB_CUDA(cudaLaunchKernelEx(&cfg, kyb::paged_attn_join_kernel<__nv_bfloat16, 64>, c.p, ctas, block));
-        else KYB_CUDA(cudaLaunchKernelEx(&cfg, kyb::paged_attn_join_kernel<__nv_bfloat16, 128>, c.p, ctas, block));
-    }
+    if (few) KYB_CUDA(cudaLaunchKernelEx(&cfg, kyb::paged_attn_join_kernel<T, D, 4, 4>, c.p, ctas, block));
+    else KYB_CUDA(cudaLaunchKernelEx(&cfg, kyb::paged_attn_join_kernel<T, D, 8, 1>, c.p, ctas, block));
     return kyb_launch_check("paged_attn_join");
+}
+
+int kyb_attn_join(const KybAttnCall& c, int ctas, int block) {
+    if (c.dtype == 1) return c.d == 64 ? launch_join<__half, 64>(c, ctas, block) : launch_join<__half, 128>(c, ctas, block);
+    return c.d == 64 ? launch_join<__nv_bfloat16, 64>(c, ctas, block) : launch_join<__nv_bfloat16, 128>(c, ctas, block);
 }
