@@ -184,9 +184,10 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_release_kernel(int* lens,
 // Token t at position m: each pair (a, b) of a query or key head's first `rot` values becomes s (a cos f - b sin f, b cos f + a sin f) with f = m inv_freq[i]; pairs
 // are (2 i, 2 i + 1) or (i, i + rot / 2). Keys (turned) and values go to the cache at the token's slot; queries to q_out. Far positions: f reaches 10^6 and more,
 // where 32 bits hold it to 0.06 only, so the product and its reduction to [-pi, pi] are made in 64 bits, sine and cosine of the rest in 32.
-// Bound by HBM: every element is read and written once, 16 bytes at a time (8191 tokens of 64 / 8 heads of 128: 56.5 us = 5.9 TB/s; 64 tokens 2.6 us). A CTA makes the rot / 2 pairs of sine and cosine of its token once in shared memory and
-// serves all of the token's heads with them; few tokens are cut into parts of the heads so that every SM has a CTA.
-constexpr int RP_THREADS = 256;
+// Bound by HBM: every element is read and written once, 16 bytes at a time (8191 tokens of 64 / 8 heads of 128: 57 us = 5.9 TB/s, 55 with neighbours paired; 64 tokens 2.8 us).
+// A CTA makes the rot / 2 pairs of sine and cosine of its token once in shared memory and serves all of the token's heads with them; few tokens are cut into parts of the
+// heads so that every SM has a CTA. Loads made before the angles (57 -> 66 us) and angles laid out without bank conflicts (57 -> 64) were slower.
+constexpr int RP_THREADS = 256;                                          // at most
 
 struct RopeParams {
     const uint8_t *q, *k, *v;                // 16-bit elements
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(RP_THREADS) rope_append_kernel(const RopeParam
     const int64_t t = blockIdx.x;
     const int pos = p.positions[t], slot = p.hkv ? p.slots[t] : -1;
     if (pos < 0) return;                                                  // a row behind the last request: nothing of it is read or written
-    for (int i = threadIdx.x; i < p.rot / 2; i += RP_THREADS) {
+    for (int i = threadIdx.x; i < p.rot / 2; i += blockDim.x) {
         const double f = (double)pos * (double)p.inv[i], turns = rint(f * 0.15915494309189533577);
         const double r = fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.283185307179586477, f));
         float s, c;
@@ -233,49 +234,39 @@ __global__ void __launch_bounds__(RP_THREADS) rope_append_kernel(const RopeParam
     const int half = p.rot / 2;
     const bool stored = slot >= 0 && (slot >> p.page_log2) < p.pages;
     const int64_t at = stored ? slot >> p.page_log2 : 0, off = stored ? (int64_t)(slot & ((1 << p.page_log2) - 1)) * p.d * 2 : 0;
-    // units of a turned head: 16-byte pieces of its plain part, and the turned part's pieces (INTER: one piece each; else two pieces half a turn apart)
-    const int turned = INTER ? p.rot / 8 : p.rot / 16, per_head = turned + (p.d - p.rot) / 8, per_v = p.d / 8;
+    // a unit is two 16-byte pieces, half of the turned part, of the plain part or of the values apart (the last one of an odd number is alone)
+    const int turned = p.rot / 16, plain = (p.d - p.rot) / 8, per_head = turned + (plain + 1) / 2, all = p.d / 8, per_v = (all + 1) / 2;
     const int units_t = (p.hq + p.hkv) * per_head, units = units_t + p.hkv * per_v;
-    for (int u = blockIdx.y * RP_THREADS + threadIdx.x; u < units; u += p.parts * RP_THREADS) {
-        if (u >= units_t) {
-            if (!stored) continue;
-            const int h = (u - units_t) / per_v, x = ((u - units_t) - h * per_v) * 16;
-            *reinterpret_cast<uint4*>(p.vc + at * p.vc_p + h * p.vc_h + off + x) = *reinterpret_cast<const uint4*>(p.v + t * p.v_t + h * p.v_h + x);
+    for (int u = blockIdx.y * blockDim.x + threadIdx.x; u < units; u += p.parts * blockDim.x) {
+        const bool value = u >= units_t;
+        const int h = value ? (u - units_t) / per_v : u / per_head, e = value ? u - units_t - h * per_v : u - h * per_head;
+        const bool query = !value && h < p.hq;
+        if (!query && !stored) continue;
+        const uint8_t* src = value ? p.v + t * p.v_t + h * p.v_h : query ? p.q + t * p.q_t + h * p.q_h : p.k + t * p.k_t + (h - p.hq) * p.k_h;
+        uint8_t* dst = value ? p.vc + at * p.vc_p + h * p.vc_h + off : query ? p.qo + t * p.qo_t + h * p.qo_h : p.kc + at * p.kc_p + (h - p.hq) * p.kc_h + off;
+        if (value || e >= turned) {
+            const int n = value ? all : plain, far = (n + 1) / 2, i = value ? e : e - turned, x = (value ? 0 : p.rot * 2) + i * 16, y = x + far * 16;
+            const bool two = i + far < n;
+            const uint4 w = *reinterpret_cast<const uint4*>(src + x);
+            uint4 z = w;
+            if (two) z = *reinterpret_cast<const uint4*>(src + y);
+            *reinterpret_cast<uint4*>(dst + x) = w;
+            if (two) *reinterpret_cast<uint4*>(dst + y) = z;
             continue;
         }
-        const int h = u / per_head, e = u - h * per_head;
-        const bool query = h < p.hq;
-        if (!query && !stored) continue;
-        const uint8_t* src = query ? p.q + t * p.q_t + h * p.q_h : p.k + t * p.k_t + (h - p.hq) * p.k_h;
-        uint8_t* dst = query ? p.qo + t * p.qo_t + h * p.qo_h : p.kc + at * p.kc_p + (h - p.hq) * p.kc_h + off;
-        if (e >= turned) {                                                // a piece that is not turned
-            const int x = p.rot * 2 + (e - turned) * 16;
-            *reinterpret_cast<uint4*>(dst + x) = *reinterpret_cast<const uint4*>(src + x);
-        } else if (INTER) {
-            uint4 w = *reinterpret_cast<const uint4*>(src + e * 16);
-            uint32_t* q = reinterpret_cast<uint32_t*>(&w);
+        const int x = e * 16, y = half * 2 + x;
+        uint4 w = *reinterpret_cast<const uint4*>(src + x), z = *reinterpret_cast<const uint4*>(src + y);
+        uint32_t *q = reinterpret_cast<uint32_t*>(&w), *r = reinterpret_cast<uint32_t*>(&z);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float2 ab = Pair<T>::get(q[j]);
-                const float2 c = cs[e * 4 + j];
-                turn(ab.x, ab.y, c.x, c.y);
-                q[j] = Pair<T>::put(ab.x, ab.y);
-            }
-            *reinterpret_cast<uint4*>(dst + e * 16) = w;
-        } else {
-            uint4 w = *reinterpret_cast<const uint4*>(src + e * 16), z = *reinterpret_cast<const uint4*>(src + half * 2 + e * 16);
-            uint32_t *q = reinterpret_cast<uint32_t*>(&w), *r = reinterpret_cast<uint32_t*>(&z);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float2 a = Pair<T>::get(q[j]), b = Pair<T>::get(r[j]);
-                const float2 c0 = cs[e * 8 + 2 * j], c1 = cs[e * 8 + 2 * j + 1];
-                turn(a.x, b.x, c0.x, c0.y);
-                turn(a.y, b.y, c1.x, c1.y);
-                q[j] = Pair<T>::put(a.x, a.y), r[j] = Pair<T>::put(b.x, b.y);
-            }
-            *reinterpret_cast<uint4*>(dst + e * 16) = w;
-            *reinterpret_cast<uint4*>(dst + half * 2 + e * 16) = z;
+        for (int j = 0; j < 4; ++j) {
+            float2 a = Pair<T>::get(q[j]), b = Pair<T>::get(r[j]);
+            const float2 c0 = cs[INTER ? e * 4 + j : e * 8 + 2 * j], c1 = cs[INTER ? half / 2 + e * 4 + j : e * 8 + 2 * j + 1];
+            if (INTER) turn(a.x, a.y, c0.x, c0.y), turn(b.x, b.y, c1.x, c1.y);
+            else turn(a.x, b.x, c0.x, c0.y), turn(a.y, b.y, c1.x, c1.y);
+            q[j] = Pair<T>::put(a.x, a.y), r[j] = Pair<T>::put(b.x, b.y);
         }
+        *reinterpret_cast<uint4*>(dst + x) = w;
+        *reinterpret_cast<uint4*>(dst + y) = z;
     }
 }
 
@@ -352,18 +343,21 @@ extern "C" int kyb_rope_append(const kyb_rope_append_args* a, void* stream) {
     p.page_log2 = 0;
     while (hkv && (1 << p.page_log2) < page) ++p.page_log2;
     p.hq = hq, p.hkv = hkv, p.d = d, p.rot = rot, p.mscale = mscale;
-    const int turned = interleaved ? rot / 8 : rot / 16, units = (hq + hkv) * (turned + (d - rot) / 8) + hkv * (d / 8);
+    const int units = (hq + hkv) * (rot / 16 + ((d - rot) / 8 + 1) / 2) + hkv * ((d / 8 + 1) / 2);
     int parts = 1;                                                        // parts of a token's heads: until every SM has two CTAs or a thread has one unit
     while (tokens * parts < 296 && parts * kyb::RP_THREADS < units) parts *= 2;
     p.parts = parts;
+    // as many threads as a CTA's units fill in equal turns (8191 tokens of 8 / 1 heads of 128, 80 units: 18 us by 256 threads, 12.3 by 96)
+    const int share = (units + parts - 1) / parts, turns = (share + kyb::RP_THREADS - 1) / kyb::RP_THREADS;
+    const int threads = std::max(64, ((share + turns - 1) / turns + 31) / 32 * 32);
     const dim3 grid((unsigned)tokens, (unsigned)parts);
     cudaStream_t st = (cudaStream_t)stream;
     if (dtype == 1) {
-        if (interleaved) kyb::rope_append_kernel<__half, true><<<grid, kyb::RP_THREADS, 0, st>>>(p);
-        else kyb::rope_append_kernel<__half, false><<<grid, kyb::RP_THREADS, 0, st>>>(p);
+        if (interleaved) kyb::rope_append_kernel<__half, true><<<grid, threads, 0, st>>>(p);
+        else kyb::rope_append_kernel<__half, false><<<grid, threads, 0, st>>>(p);
     } else {
-        if (interleaved) kyb::rope_append_kernel<__nv_bfloat16, true><<<grid, kyb::RP_THREADS, 0, st>>>(p);
-        else kyb::rope_append_kernel<__nv_bfloat16, false><<<grid, kyb::RP_THREADS, 0, st>>>(p);
+        if (interleaved) kyb::rope_append_kernel<__nv_bfloat16, true><<<grid, threads, 0, st>>>(p);
+        else kyb::rope_append_kernel<__nv_bfloat16, false><<<grid, threads, 0, st>>>(p);
     }
     return kyb_launch_check("rope_append");
 }
