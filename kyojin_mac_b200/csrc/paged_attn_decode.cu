@@ -6,8 +6,8 @@
 // weights around in registers (movmatrix) and accumulates O^T = V^T P^T. tcgen05 would compute 128 rows for 8; here the tensor work is a sixth of the time the bytes take.
 // The reference maximum of a row moves only when a score passes it by 2^8 (a warp vote), so the usual stage needs no shuffle and no rescaling.
 // Measured, 64 / 8 heads of 128: 64 sequences of 1000 to 16000 tokens 329 us = 6.7 TB/s, one of 778 tokens 9.8 us (both launches); counters: DRAM 1.01 x the necessary bytes,
-// issue slots 17 %. Requests of up to 16 rows come here, since their loop needs no more than the bytes' time; with 24 rows (three tokens of 8 heads, 8000 cached) the prefill
-// kernel takes 393 us for 64 requests and this one would re-read the keys for every 16 rows.
+// issue slots 17 %. Requests of up to 16 rows come here, since their loop needs no more than the bytes' time; with 32 rows (four tokens of 8 heads, 8000 cached) the prefill
+// kernel takes 368 us for 64 requests, where the bytes take 320, and this one would read the keys again for every 16 rows.
 // Places that no row sees may hold anything: their weights are selected, not multiplied, to 0, and their values are cleared in the V fragments.
 #include <algorithm>
 

@@ -199,6 +199,16 @@ def test_chunk_heads(hq, hkv):
     _attend([150, 40, 391], [70, 40, 9], hq, hkv, 64, 32, F16, seed=hq)
 
 
+@pytest.mark.parametrize("b,most", [(161, 1), (700, 2), (400, 40), (900, 9)])
+def test_more_requests_than_threads(b, most):
+    """Batches beyond what one pass of a CTA's threads over the lengths takes, requests without rows and without keys among them."""
+    r = random.Random(b)
+    qn = [r.choice((0, 1, 1, r.randint(1, most))) for _ in range(b)]
+    qn[3] = most
+    kv = [n + r.choice((0, r.randint(0, 40), r.randint(0, 200))) if r.random() < 0.9 else 0 for n in qn]
+    _attend(kv, qn, 4, 1, 64, 16, F16, seed=b)
+
+
 def test_long_contexts_are_split():
     _attend([9001], [1], 8, 1, 128, 64, F16, seed=1)
     _attend([6000, 5], [1, 1], 4, 2, 64, 128, BF16, seed=2)
