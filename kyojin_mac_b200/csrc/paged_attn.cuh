@@ -207,10 +207,10 @@ struct KybAttnCall {
     int d, dtype, page, sms;
     cudaStream_t st;
 };
-// an upper bound of the units that the kernels deal out: row blocks (each request's last may be a part) x heads x tiles of a full table row and an item's extra
-static inline bool kyb_attn_units_fit(const KybAttnCall& c, int block, int tile) {
+// an upper bound of the units that the kernels deal out: row blocks (each request's last may be a part) x heads x tiles of a full table row and an item's extra; 0 from 2^31 on
+static inline int64_t kyb_attn_units(const KybAttnCall& c, int block, int tile) {
     const int64_t blocks = c.tokens * c.p.group / block + c.p.batch, tiles = (int64_t)c.p.cap / tile + 8;
-    return blocks * c.p.hkv < (1ll << 31) / tiles;
+    return blocks * c.p.hkv < (1ll << 31) / tiles ? blocks * c.p.hkv * tiles : 0;
 }
 // rows a request may bring for the decode kernel; beyond, the prefill kernel
 constexpr int KYB_DECODE_ROWS = 16;

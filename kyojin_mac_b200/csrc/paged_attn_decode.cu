@@ -438,8 +438,9 @@ int launch_decode(KybAttnCall& c, void* ws) {
     using S = kyb::DecodeShape<D, NT>;
     auto kern = kyb::paged_attn_decode_kernel<T, D, NT>;
     if (int rc = kyb_allow_smem((const void*)kern)) return rc;
-    KYB_REQUIRE(kyb_attn_units_fit(c, S::ROWS, kyb::DC_TILE), "more than 2^31 key tiles in one call: split it");
-    const int ctas = DC_PER_SM * c.sms, piece = std::min(c.page, kyb::DC_TILE);
+    const int64_t units = kyb_attn_units(c, S::ROWS, kyb::DC_TILE);
+    KYB_REQUIRE(units, "more than 2^31 key tiles in one call: split it");
+    const int ctas = (int)std::min<int64_t>(DC_PER_SM * c.sms, units), piece = std::min(c.page, kyb::DC_TILE);
     CUtensorMap mk, mv;
     if (int rc = kyb_make_cache_map(&mk, c.k, c.dtype, c.p.pages, c.p.hkv, c.page, D, c.k_p, c.k_h, piece, D / 64)) return rc;
     if (int rc = kyb_make_cache_map(&mv, c.v, c.dtype, c.p.pages, c.p.hkv, c.page, D, c.v_p, c.v_h, piece, D / 64)) return rc;

@@ -105,8 +105,8 @@ __device__ __forceinline__ int scan_block(int v, int* sums, int& total) {
     }
     return v;
 }
-// units of up to PF_THREADS requests from r0 on, of all heads: the row blocks of all of them are shared among the threads
-__device__ __forceinline__ int count_chunk(const AttnParams& p, int block, int r0, RunFinder& f, int& end) {
+// rows, keys and (scanned) row blocks of up to PF_THREADS requests from r0 on; gives the number of their row blocks
+__device__ __forceinline__ int load_chunk(const AttnParams& p, int block, int r0, RunFinder& f) {
     const int tid = threadIdx.x, n = min(PF_THREADS, p.batch - r0);
     int nb = 0;
     if (tid < n) {
@@ -114,9 +114,15 @@ __device__ __forceinline__ int count_chunk(const AttnParams& p, int block, int r
         f.tokens[tid] = request_rows(p, r0 + tid, base), f.kv[tid] = request_keys(p, r0 + tid);
         nb = row_blocks(p, f.tokens[tid], block);
     }
-    f.units[tid] = 0;
     int all;
     f.blocks_end[tid] = scan_block(nb, f.sums[0], all);
+    return all;
+}
+// their units, of all heads: the row blocks of all of them are shared among the threads
+__device__ __forceinline__ int count_chunk(const AttnParams& p, int block, int r0, RunFinder& f, int& end) {
+    const int tid = threadIdx.x, n = min(PF_THREADS, p.batch - r0);
+    f.units[tid] = 0;
+    const int all = load_chunk(p, block, r0, f);
     __syncthreads();
     for (int i0 = tid & ~31; i0 < all; i0 += PF_THREADS) {                   // whole numbers: the order of the additions does not matter
         const int i = min(i0 + (tid & 31), all - 1), r = first_end_above(f.blocks_end, n, i), rb = i - (r ? f.blocks_end[r - 1] : 0);
@@ -132,17 +138,40 @@ __device__ __forceinline__ int count_chunk(const AttnParams& p, int block, int r
     end = scan_block(f.units[tid], f.sums[1], total);
     return total;
 }
+// a run that starts x units into row block rb of request r (whose items have `one` units each) and has `length` units
+__device__ __forceinline__ void enter_run(const AttnParams& p, int block, Cursor& k, int r, int rb, int x, int one, int length) {
+    k.r = r, k.rb = rb, k.left = length;
+    k.load(p, block, PF_TILE);
+    k.h = x / one;
+    k.at = PrefillRuns::enter(k.s, x - k.h * one, k.left);
+    if (k.at == k.s.n) k.next(p, block, PF_TILE);
+}
 // The run of tiles of CTA blockIdx.x, into f.run
 __device__ __forceinline__ void find_run_wide(const AttnParams& p, int block, RunFinder& f) {
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, c = blockIdx.x;
+    if (tid == 0) f.run.left = 0, f.request = 0, f.at = 0;
+    if (p.batch <= PF_THREADS) {
+        const int all = load_chunk(p, block, 0, f);
+        __syncthreads();
+        if (all <= PF_THREADS) {                                             // a row block a thread: one more scan gives the sums and the place
+            const int r = tid < all ? first_end_above(f.blocks_end, p.batch, tid) : 0, rb = tid - (r ? f.blocks_end[r - 1] : 0);
+            const int one = tid < all ? PrefillRuns::units(key_span(p, f.tokens[r], f.kv[r], block, rb, PF_TILE)) : 0, n = one * p.hkv;
+            int total;
+            const int e = scan_block(n, f.sums[1], total), ctas = min((int)gridDim.x, total);
+            if (c >= ctas) return;
+            const int u0 = run_border(total, ctas, c);
+            if (n && u0 >= e - n && u0 < e) enter_run(p, block, f.run, r, rb, u0 - (e - n), one, run_border(total, ctas, c + 1) - u0);
+            return;
+        }
+        __syncthreads();
+    }
     int total = 0, end = 0, mine = 0;
     for (int r0 = 0; r0 < p.batch; r0 += PF_THREADS) {
         if (r0) __syncthreads();
         mine = count_chunk(p, block, r0, f, end), total += mine;
     }
-    const int ctas = min((int)gridDim.x, total), c = blockIdx.x;
+    const int ctas = min((int)gridDim.x, total);
     const int u0 = c < ctas ? run_border(total, ctas, c) : 0, u1 = c < ctas ? run_border(total, ctas, c + 1) : 0;
-    if (tid == 0) f.run.left = 0, f.request = 0, f.at = 0;
     if (u1 == u0) return;
     __syncthreads();
     int before = 0;
@@ -164,15 +193,7 @@ __device__ __forceinline__ void find_run_wide(const AttnParams& p, int block, Ru
         const int rb = b0 + tid, one = rb < nb ? PrefillRuns::units(key_span(p, tokens, kv, block, rb, PF_TILE)) : 0, n = one * p.hkv;
         int all;
         const int e = before + scan_block(n, f.sums[b0 / PF_THREADS & 1], all);
-        if (n && at >= e - n && at < e) {
-            Cursor& k = f.run;
-            const int x = at - (e - n);
-            k.r = r, k.rb = rb, k.left = u1 - u0;
-            k.load(p, block, PF_TILE);
-            k.h = x / one;
-            k.at = PrefillRuns::enter(k.s, x - k.h * one, k.left);
-            if (k.at == k.s.n) k.next(p, block, PF_TILE);
-        }
+        if (n && at >= e - n && at < e) enter_run(p, block, f.run, r, rb, at - (e - n), one, u1 - u0);
         before += all;
     }
 }
@@ -620,8 +641,10 @@ int launch_prefill(KybAttnCall& c, void* ws) {
     using S = kyb::PrefillShape<D>;
     auto kern = kyb::paged_attn_prefill_kernel<T, D>;
     if (int rc = kyb_allow_smem((const void*)kern)) return rc;
-    const int ctas = c.sms, piece = std::min(c.page, kyb::PF_TILE), qtoks = 128 / c.p.group;
-    KYB_REQUIRE(kyb_attn_units_fit(c, 2 * qtoks * c.p.group, kyb::PF_TILE), "more than 2^31 key tiles in one call: split it");
+    const int piece = std::min(c.page, kyb::PF_TILE), qtoks = 128 / c.p.group;
+    const int64_t units = kyb_attn_units(c, 2 * qtoks * c.p.group, kyb::PF_TILE);
+    KYB_REQUIRE(units, "more than 2^31 key tiles in one call: split it");
+    const int ctas = (int)std::min<int64_t>(c.sms, units);
     CUtensorMap mq, mk, mv;
     if (int rc = make_query_map(&mq, c, qtoks)) return rc;
     if (int rc = kyb_make_cache_map(&mk, c.k, c.dtype, c.p.pages, c.p.hkv, c.page, D, c.k_p, c.k_h, piece, 1)) return rc;
