@@ -22,7 +22,7 @@ struct AttnParams {
     const int* cu_q;
     int64_t ld_table;
     int batch, tokens, hq, hkv, group, page_log2, pages, cap; // tokens: rows of q; cap: tokens that a row of the table can hold
-    int block_tokens;
+    int block_tokens;                                         // tokens of a row block, where it is made of whole ones (0: it is not)
     int window, sinks;                                        // window 0: none
     float scale2;                                             // scale log2(e)
     unsigned int* status;

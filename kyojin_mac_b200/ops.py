@@ -16,9 +16,6 @@ from .layout import FMT_ID, padded_rows
 _raw_stream, _cur_device = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None)
 
 
-_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
-
-
 def _stream() -> int:
     if _raw_stream is None or not torch.cuda.is_initialized():
         return torch.cuda.current_stream().cuda_stream
@@ -773,8 +770,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     need, sizes = known
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    # scratch: the stream's own, or inside a capture the call's, so that captured graphs that replay side by side share nothing
-    ws = q.new_empty((need + 1) // 2) if _capturing() else workspace(q.device, need)
+    # the call's own scratch: captured graphs that replay side by side share nothing, nor do calls of two threads on one stream, whose launches may interleave
+    ws = q.new_empty((need + 1) // 2)
     rc = _lib.lib().kyb_paged_attention(_lib.PAGED_ATTENTION_ARGS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), kv_lens.data_ptr(), cu_q.data_ptr(), out.data_ptr(),
                                                                        ws.data_ptr(), *sizes, q.shape[2] ** -0.5 if scale is None else scale), _stream())
     if rc:

@@ -437,8 +437,9 @@ def test_row_offsets_out_of_order(qn):
     ops.check_device_status()
 
 
-def test_another_stream_and_threads():
-    """Calls on side streams, from two host threads at once, give what calls in a row give."""
+@pytest.mark.parametrize("one_stream", [False, True])
+def test_another_stream_and_threads(one_stream):
+    """Calls on side streams, from two host threads at once (on streams of their own or on one), give what calls in a row give."""
     import threading
     k, v, table = R.pool([700, 300], 32, 2, 128, F16, 24)
     lens = _i32([700, 300])
@@ -446,9 +447,10 @@ def test_another_stream_and_threads():
     want = [ops.paged_attention(q, k, v, table, lens, cu, n) for q, cu, n in jobs]
     torch.cuda.synchronize()
     got = [[None] * 4 for _ in range(2)]
+    shared = torch.cuda.Stream()
 
     def work(who):
-        with torch.cuda.stream(torch.cuda.Stream()):
+        with torch.cuda.stream(shared if one_stream else torch.cuda.Stream()):
             for _ in range(20):
                 for i, (q, cu, n) in enumerate(jobs):
                     got[who][i] = ops.paged_attention(q, k, v, table, lens, cu, n)
