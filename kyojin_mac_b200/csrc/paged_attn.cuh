@@ -164,18 +164,12 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, fl
 // tensor map of a cache [pages][heads][page][d] of 16-bit values: {64 values, token, half, head, page}, boxes of `box_tokens` tokens and `box_halves` halves
 static inline int kyb_make_cache_map(CUtensorMap* tm, const void* base, int dtype, int64_t pages, int heads, int page, int d, int64_t page_stride, int64_t head_stride, int box_tokens,
                                      int box_halves) {
-    kyb_encode_tiled_fn enc = kyb_get_encode_tiled();
-    if (!enc) {
-        kyb_set_error("cuTensorMapEncodeTiled is not available from this driver");
-        return KYB_ECUDA;
-    }
     if (heads == 1) head_stride = (int64_t)page * d;                        // the stride of a dimension of one is never used: any valid one
     if (pages == 1) page_stride = head_stride * heads;
     const cuuint64_t dims[5] = {64, (cuuint64_t)page, (cuuint64_t)(d / 64), (cuuint64_t)heads, (cuuint64_t)pages};
     const cuuint64_t strides[4] = {(cuuint64_t)d * 2, 128, (cuuint64_t)head_stride * 2, (cuuint64_t)page_stride * 2};
-    const cuuint32_t box[5] = {64, (cuuint32_t)box_tokens, (cuuint32_t)box_halves, 1, 1}, estr[5] = {1, 1, 1, 1, 1};
-    const CUresult r = enc(tm, dtype == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(base), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const cuuint32_t box[5] = {64, (cuuint32_t)box_tokens, (cuuint32_t)box_halves, 1, 1};
+    const CUresult r = kyb_encode_map(tm, dtype == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (r != CUDA_SUCCESS) {
         kyb_set_error("cuTensorMapEncodeTiled failed with CUresult %d (cache %p: %lld pages, %d heads, %d tokens of %d values, strides %lld, %lld)", (int)r, base, (long long)pages, heads, page,
                       d, (long long)page_stride, (long long)head_stride);

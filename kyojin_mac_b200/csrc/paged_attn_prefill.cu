@@ -618,18 +618,12 @@ namespace {
 
 // queries [tokens][kv heads][group][d]: {64 values, half, head of the group, kv head, token}, boxes of all heads of a group and `qtoks` tokens
 int make_query_map(CUtensorMap* tm, const KybAttnCall& c, int qtoks) {
-    kyb_encode_tiled_fn enc = kyb_get_encode_tiled();
-    if (!enc) {
-        kyb_set_error("cuTensorMapEncodeTiled is not available from this driver");
-        return KYB_ECUDA;
-    }
     const kyb::AttnParams& p = c.p;
     const int64_t head = p.hq == 1 ? c.d : p.q_h, token = c.tokens == 1 ? (int64_t)c.d * p.hq : p.q_t;       // the stride of a dimension of one is never used: any valid one
     const cuuint64_t dims[5] = {64, (cuuint64_t)(c.d / 64), (cuuint64_t)p.group, (cuuint64_t)p.hkv, (cuuint64_t)c.tokens};
     const cuuint64_t strides[4] = {128, (cuuint64_t)head * 2, (cuuint64_t)head * 2 * (cuuint64_t)p.group, (cuuint64_t)token * 2};
-    const cuuint32_t box[5] = {64, 1, (cuuint32_t)p.group, 1, (cuuint32_t)qtoks}, estr[5] = {1, 1, 1, 1, 1};
-    const CUresult r = enc(tm, c.dtype == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<uint8_t*>(p.q), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const cuuint32_t box[5] = {64, 1, (cuuint32_t)p.group, 1, (cuuint32_t)qtoks};
+    const CUresult r = kyb_encode_map(tm, c.dtype == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, p.q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (r != CUDA_SUCCESS) {
         kyb_set_error("cuTensorMapEncodeTiled failed with CUresult %d (queries %p: %lld tokens, %d x %d heads of %d, strides %lld, %lld)", (int)r, (const void*)p.q, (long long)c.tokens, p.hkv,
                       p.group, c.d, (long long)token, (long long)head);

@@ -21,22 +21,31 @@ static inline kyb_encode_tiled_fn kyb_get_encode_tiled() {
     return fn;
 }
 
+// Encodes a map. A host thread whose first CUDA call this is has no current context yet (the runtime binds one at its first call that needs it, the driver's encoder does
+// not): cudaSetDevice on the thread's device binds it, inside a stream capture too, and the map is encoded again.
+static inline CUresult kyb_encode_map(CUtensorMap* tm, CUtensorMapDataType dt, cuuint32_t rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                                      CUtensorMapSwizzle swizzle) {
+    kyb_encode_tiled_fn enc = kyb_get_encode_tiled();
+    if (!enc) return CUDA_ERROR_NOT_FOUND;
+    const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+    auto encode = [&]() {
+        return enc(tm, dt, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = encode();
+    int dev = 0;
+    if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+    return r;
+}
+
 // 2-D row-major tensor [rows, cols] of `elem_bytes`-wide elements, row stride `ld_bytes`; box [box_rows, box_cols]; 128-byte swizzle by default
 // (box_cols * elem_bytes must equal the swizzle width). Out-of-range parts of a box are filled with zeros on loads and dropped on stores.
 static inline int kyb_make_tmap_2d(CUtensorMap* tm, CUtensorMapDataType dt, int elem_bytes, const void* base, uint64_t rows, uint64_t cols, uint64_t ld_bytes,
                                    uint32_t box_rows, uint32_t box_cols, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
-    kyb_encode_tiled_fn enc = kyb_get_encode_tiled();
-    if (!enc) {
-        kyb_set_error("cuTensorMapEncodeTiled is not available from this driver");
-        return KYB_ECUDA;
-    }
     const cuuint64_t dims[2] = {cols, rows};
     const cuuint64_t strides[1] = {ld_bytes};
     const cuuint32_t box[2] = {box_cols, box_rows};
-    const cuuint32_t estr[2] = {1, 1};
     (void)elem_bytes;
-    const CUresult r = enc(tm, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUresult r = kyb_encode_map(tm, dt, 2, base, dims, strides, box, swizzle);
     if (r != CUDA_SUCCESS) {
         kyb_set_error("cuTensorMapEncodeTiled failed with CUresult %d (base %p rows %llu cols %llu ld %llu box %u x %u)", (int)r, base, (unsigned long long)rows,
                       (unsigned long long)cols, (unsigned long long)ld_bytes, box_rows, box_cols);

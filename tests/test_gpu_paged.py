@@ -459,3 +459,16 @@ def test_another_stream_and_threads(one_stream):
     [t.start() for t in threads], [t.join() for t in threads]
     assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
 
+
+def test_first_cuda_call_of_a_thread():
+    """Both kernels as the first CUDA call that a host thread makes."""
+    import threading
+    k, v, table = R.pool([300], 32, 2, 128, F16, 25)
+    lens, got = _i32([300]), {}
+    jobs = {n: (torch.randn((n, 8, 128), device="cuda").to(F16), _i32([0, n])) for n in (1, 50)}
+    outs = {n: torch.zeros_like(q) for n, (q, _) in jobs.items()}
+    torch.cuda.synchronize()
+    for n, (q, cu) in jobs.items():
+        t = threading.Thread(target=lambda: got.update({n: ops.paged_attention(q, k, v, table, lens, cu, n, out=outs[n])}))
+        t.start(), t.join()
+        assert torch.equal(got[n], ops.paged_attention(q, k, v, table, lens, cu, n))
