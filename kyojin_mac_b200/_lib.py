@@ -111,10 +111,11 @@ class PeerOut(C.Structure):
 
 _pp = C.POINTER(PeerOut)
 
-# argument blocks of the paged-cache entries (kyb_*_args): pointers, then int64 fields, then a double where there is one; packed by struct in native order
-PAGED_STEP_ARGS = struct.Struct("=12Q6q")
-ROPE_APPEND_ARGS = struct.Struct("=9Q21qd")
-PAGED_ATTENTION_ARGS = struct.Struct("=8Q22qd")
+# argument blocks of the paged-cache entries (kyb_*_args): pointers, then int64 fields, then a double where there is one; packed by struct in native order. The pointers change from
+# call to call, the rest hardly ever: a caller may pack the two apart and join the bytes.
+PAGED_STEP_ARGS, PAGED_STEP_SPLIT = struct.Struct("=12Q6q"), (struct.Struct("=12Q"), struct.Struct("=6q"))
+ROPE_APPEND_ARGS, ROPE_APPEND_SPLIT = struct.Struct("=9Q21qd"), (struct.Struct("=9Q"), struct.Struct("=21qd"))
+PAGED_ATTENTION_ARGS, PAGED_ATTENTION_SPLIT = struct.Struct("=8Q22qd"), (struct.Struct("=8Q"), struct.Struct("=22qd"))
 
 SIGNATURES = {
     "kyb_version": (_int, []),

@@ -590,7 +590,7 @@ def paged_step(table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor, 
             raise ValueError("the free list is an array with room for a page at least, rows not negative")
         sizes = [b + 1, b, rows, rows, 1] + ([] if in_place else [b, 1])
         offs = [4 * sum(sizes[:i]) for i in range(len(sizes))]
-        known = _remember(key, (sum(sizes), sizes, offs, (free_pages.shape[0], max(table.stride(0), cols), b, cols, page, rows)))
+        known = _remember(key, (sum(sizes), sizes, offs, _lib.PAGED_STEP_SPLIT[1].pack(free_pages.shape[0], max(table.stride(0), cols), b, cols, page, rows)))
     if dev != torch.cuda.current_device() if _cur_device is None else dev != _cur_device():
         with torch.cuda.device(dev):
             return paged_step(table, lens, new_lens, free_pages, free_count, page, rows, in_place)
@@ -600,8 +600,8 @@ def paged_step(table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor, 
     cu, kv, pos, slots, refused, *more = buf.split_with_sizes(sizes)
     out_lens, out_count = (lens, free_count) if in_place else more
     out_lens_p, out_count_p = (lens_p, count_p) if in_place else (at + offs[5], at + offs[6])
-    rc = _lib.lib().kyb_paged_step(_lib.PAGED_STEP_ARGS.pack(lens_p, new_lens.data_ptr(), free_pages.data_ptr(), count_p, table.data_ptr(), at, at + offs[1], at + offs[2], at + offs[3], out_lens_p,
-                                                             out_count_p, at + offs[4], *numbers), _stream())
+    rc = _lib.lib().kyb_paged_step(_lib.PAGED_STEP_SPLIT[0].pack(lens_p, new_lens.data_ptr(), free_pages.data_ptr(), count_p, table.data_ptr(), at, at + offs[1], at + offs[2], at + offs[3],
+                                                                 out_lens_p, out_count_p, at + offs[4]) + numbers, _stream())
     if rc:
         _lib.check(rc)
     return PagedStep(cu, kv, pos, slots, out_lens, out_count, refused)
@@ -661,7 +661,7 @@ def rope_frequencies(rot: int, base: float = 10000.0, scaling: dict | None = Non
     return inv.to(torch.float32).to(device), mscale
 
 
-def _rope_check(key, q, k, v, positions, slots, inv_freq, kc, vc, out):
+def _rope_check(key, q, k, v, positions, slots, inv_freq, kc, vc, interleaved, mscale, out):
     _place(*(t for t in (q, k, v, positions, slots, inv_freq, kc, vc, out) if t is not None))
     _heads(q, "q"), _i32(positions, "positions", q.shape[0])
     if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
@@ -680,35 +680,37 @@ def _rope_check(key, q, k, v, positions, slots, inv_freq, kc, vc, out):
         ks, vs, kcs, vcs = k.stride()[:2], v.stride()[:2], kc.stride()[:2], vc.stride()[:2]
         pages, hkv, page = kc.shape[:3]
     os_ = (hq * d, d) if out is None else out.stride()[:2]
-    return _remember(key, (*q.stride()[:2], *ks, *vs, *os_, *kcs, *vcs, T, hq, hkv, d, 2 * inv_freq.shape[0]))
+    return _remember(key, _lib.ROPE_APPEND_SPLIT[1].pack(*q.stride()[:2], *ks, *vs, *os_, *kcs, *vcs, T, hq, hkv, d, 2 * inv_freq.shape[0], 1 if interleaved else 0, _DT[q.dtype], pages, page,
+                                                         mscale))
 
 
 def _rope_call(q, k, v, positions, slots, inv_freq, kc, vc, interleaved, mscale, out):
     """The queries turned (into `out`), keys and values into the cache where there are any."""
     dev, grad = q.get_device(), q.requires_grad
     if k is None:
-        key = (dev, q.shape, q.stride(), q.dtype, positions.shape, positions.dtype, positions.is_contiguous(), inv_freq.shape, inv_freq.dtype, positions.get_device(), inv_freq.get_device())
+        key = (dev, q.shape, q.stride(), q.dtype, positions.shape, positions.dtype, positions.is_contiguous(), inv_freq.shape, inv_freq.dtype, positions.get_device(), inv_freq.get_device(), interleaved,
+               mscale)
     else:
         grad = grad or k.requires_grad or v.requires_grad
         key = (dev, q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, positions.shape, positions.dtype, positions.is_contiguous(), slots.shape, slots.dtype,
                slots.is_contiguous(), inv_freq.shape, inv_freq.dtype, kc.shape, kc.is_contiguous() or kc.stride(), kc.dtype, vc.shape, vc.is_contiguous() or vc.stride(), vc.dtype, k.get_device(),
-               v.get_device(), positions.get_device(), slots.get_device(), inv_freq.get_device(), kc.get_device(), vc.get_device())
+               v.get_device(), positions.get_device(), slots.get_device(), inv_freq.get_device(), kc.get_device(), vc.get_device(), interleaved, mscale)
     if out is not None:
         key += (out.shape, out.stride(), out.dtype, out.get_device())
-    sizes = None if grad or not inv_freq.is_contiguous() else _passed.get(key)
-    if sizes is None:
-        sizes = _rope_check(key, q, k, v, positions, slots, inv_freq, kc, vc, out)
+    numbers = None if grad or not inv_freq.is_contiguous() else _passed.get(key)
+    if numbers is None:
+        numbers = _rope_check(key, q, k, v, positions, slots, inv_freq, kc, vc, interleaved, mscale, out)
     if dev != torch.cuda.current_device() if _cur_device is None else dev != _cur_device():
         with torch.cuda.device(dev):
             return _rope_call(q, k, v, positions, slots, inv_freq, kc, vc, interleaved, mscale, out)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    qp, pp, ip, op = q.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), out.data_ptr()
     if k is None:
-        ptrs, pages = (q.data_ptr(), 0, 0, positions.data_ptr(), 0, inv_freq.data_ptr(), out.data_ptr(), 0, 0), (0, 0)
+        ptrs = _lib.ROPE_APPEND_SPLIT[0].pack(qp, 0, 0, pp, 0, ip, op, 0, 0)
     else:
-        ptrs = (q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr(), out.data_ptr(), kc.data_ptr(), vc.data_ptr())
-        pages = kc.shape[0], kc.shape[2]
-    rc = _lib.lib().kyb_rope_append(_lib.ROPE_APPEND_ARGS.pack(*ptrs, *sizes, 1 if interleaved else 0, _DT[q.dtype], *pages, mscale), _stream())
+        ptrs = _lib.ROPE_APPEND_SPLIT[0].pack(qp, k.data_ptr(), v.data_ptr(), pp, slots.data_ptr(), ip, op, kc.data_ptr(), vc.data_ptr())
+    rc = _lib.lib().kyb_rope_append(ptrs + numbers, _stream())
     if rc:
         _lib.check(rc)
     return out
@@ -728,7 +730,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     return _rope_call(q, k, v, positions, slots, inv_freq, k_cache, v_cache, interleaved, mscale, out)
 
 
-def _attention_check(key, q, kc, vc, table, kv_lens, cu_q, max_q, window, sinks, out):
+def _attention_check(key, q, kc, vc, table, kv_lens, cu_q, max_q, scale, window, sinks, out):
     _place(*(t for t in (q, kc, vc, table, kv_lens, cu_q, out) if t is not None))
     _heads(q, "q"), _cache(kc, "k_cache"), _cache(vc, "v_cache", kc)
     (T, hq, d), (pages, hkv, page, dk) = q.shape, kc.shape
@@ -746,8 +748,8 @@ def _attention_check(key, q, kc, vc, table, kv_lens, cu_q, max_q, window, sinks,
     with torch.cuda.device(q.device):
         need = _lib.lib().kyb_paged_attention_workspace_bytes(b, T, max_q, cols, page, hq, hkv, d)
     os_ = (hq * d, d) if out is None else out.stride()[:2]
-    return _remember(key, (need, (*q.stride()[:2], *kc.stride()[:2], *vc.stride()[:2], *os_, pages, page, max(table.stride(0), cols), cols, b, T, max_q, hq, hkv, d, _DT[q.dtype], window, sinks,
-                                  need)))
+    return _remember(key, (need, _lib.PAGED_ATTENTION_SPLIT[1].pack(*q.stride()[:2], *kc.stride()[:2], *vc.stride()[:2], *os_, pages, page, max(table.stride(0), cols), cols, b, T, max_q, hq, hkv,
+                                                                    d, _DT[q.dtype], window, sinks, need, d ** -0.5 if scale is None else scale)))
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, kv_lens: torch.Tensor, cu_q: torch.Tensor, max_q: int, scale: float | None = None,
@@ -759,21 +761,21 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     dev = q.get_device()
     key = (dev, q.shape, q.is_contiguous() or q.stride(), q.dtype, k_cache.shape, k_cache.is_contiguous() or k_cache.stride(), k_cache.dtype, v_cache.shape,
            v_cache.is_contiguous() or v_cache.stride(), v_cache.dtype, table.shape, table.is_contiguous() or table.stride(), table.dtype, kv_lens.shape, kv_lens.dtype, kv_lens.is_contiguous(),
-           cu_q.shape, cu_q.dtype, cu_q.is_contiguous(), max_q, window, sinks, k_cache.get_device(), v_cache.get_device(), table.get_device(), kv_lens.get_device(), cu_q.get_device(),
+           cu_q.shape, cu_q.dtype, cu_q.is_contiguous(), max_q, scale, window, sinks, k_cache.get_device(), v_cache.get_device(), table.get_device(), kv_lens.get_device(), cu_q.get_device(),
            None if out is None else (out.shape, out.stride(), out.dtype, out.get_device()))
     known = None if q.requires_grad else _passed.get(key)
     if known is None:
-        known = _attention_check(key, q, k_cache, v_cache, table, kv_lens, cu_q, max_q, window, sinks, out)
+        known = _attention_check(key, q, k_cache, v_cache, table, kv_lens, cu_q, max_q, scale, window, sinks, out)
     if dev != torch.cuda.current_device() if _cur_device is None else dev != _cur_device():
         with torch.cuda.device(dev):
             return paged_attention(q, k_cache, v_cache, table, kv_lens, cu_q, max_q, scale, window, sinks, out)
-    need, sizes = known
+    need, numbers = known
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     # the call's own scratch: captured graphs that replay side by side share nothing, nor do calls of two threads on one stream, whose launches may interleave
     ws = q.new_empty((need + 1) // 2)
-    rc = _lib.lib().kyb_paged_attention(_lib.PAGED_ATTENTION_ARGS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), kv_lens.data_ptr(), cu_q.data_ptr(), out.data_ptr(),
-                                                                       ws.data_ptr(), *sizes, q.shape[2] ** -0.5 if scale is None else scale), _stream())
+    rc = _lib.lib().kyb_paged_attention(_lib.PAGED_ATTENTION_SPLIT[0].pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), kv_lens.data_ptr(), cu_q.data_ptr(),
+                                                                           out.data_ptr(), ws.data_ptr()) + numbers, _stream())
     if rc:
         _lib.check(rc)
     return out
