@@ -7,7 +7,8 @@
 //   10         clears values in places that no row sees (11 is idle: registers move between groups of four warps, from these four to the softmax)
 // Tensor memory: S0 | S1 | O0 | O1, 128 columns each; the weights P (16 bits) take the place of their scores S. S = Q K^T with both operands in shared memory; O += P V with
 // P in tensor memory and V as it lies in the cache (MN-major operand). The issuer's order S0(j+1) behind O0(j), S1(j+1) behind O1(j) keeps the tensor cores busy
-// with one query tile while the softmax of the other runs. A row's reference maximum moves only when a score passes it by 2^15, so O is rescaled (by the softmax warps
+// with one query tile while the softmax of the other runs; S(j+1) may overwrite P(j) without a wait in between, since one thread issues both products to the SM's one tensor
+// core, which runs them in that order. A row's reference maximum moves only when a score passes it by 2^15, so O is rescaled (by the softmax warps
 // themselves, in tensor memory) hardly ever; sums are of the unrounded weights, in 32 bits.
 // Measured, 64 / 8 heads of 128: 1024 tokens on 8192 cached ones 245 to 250 us, a prompt of 8192 tokens 910 us = 1210 TFLOP/s; 3200 clocks a pair of tiles, of which the tensor
 // cores and the special-function units are busy 2050 each.
