@@ -8,8 +8,9 @@
 // Tensor memory: S0 | S1 | O0 | O1, 128 columns each; the weights P (16 bits) take the place of their scores S. S = Q K^T with both operands in shared memory; O += P V with
 // P in tensor memory and V as it lies in the cache (MN-major operand). The issuer's order S0(j+1) behind O0(j), S1(j+1) behind O1(j) keeps the tensor cores busy
 // with one query tile while the softmax of the other runs; S(j+1) may overwrite P(j) without a wait in between, since one thread issues both products to the SM's one tensor
-// core, which runs them in that order. A row's reference maximum moves only when a score passes it by 2^15, so O is rescaled (by the softmax warps
-// themselves, in tensor memory) hardly ever; sums are of the unrounded weights, in 32 bits.
+// core, which runs them in that order. An item's last O has a barrier of its own: on the scores' one the next item's first scores, which wait for nothing of the softmax, could end
+// a second phase before a late softmax warp has seen the first, and a wait by parity would not pass any more. A row's reference maximum moves only when a score passes it by
+// 2^15, so O is rescaled (by the softmax warps themselves, in tensor memory) hardly ever; sums are of the unrounded weights, in 32 bits.
 // Measured, 64 / 8 heads of 128: 1024 tokens on 8192 cached ones 245 to 250 us, a prompt of 8192 tokens 910 us = 1210 TFLOP/s; 3200 clocks a pair of tiles, of which the tensor
 // cores and the special-function units are busy 2050 each.
 // Keys that a row does not see are masked by selection in the tiles at the borders; values in places that no row of the block sees are cleared in shared memory, since such
@@ -31,7 +32,7 @@ template <int D>
 struct PrefillShape {
     static constexpr uint32_t HALVES = D / 64, HALF = 128 * 128, TILE = HALVES * HALF;       // a tile of 128 rows: halves of 64 values, 128-byte rows
     static constexpr int SLOTS = 4 * 128 / D;                                // an even number: K in the even ones, V in the odd ones
-    static constexpr uint32_t OFF_KV = 2 * TILE, OFF_OUT = OFF_KV + SLOTS * TILE, OFF_BAR = OFF_OUT + 8 * 4096, OFF_CUR = OFF_BAR + 24 * SLOTS + 80, SMEM = OFF_CUR + 8 * sizeof(Cursor);
+    static constexpr uint32_t OFF_KV = 2 * TILE, OFF_OUT = OFF_KV + SLOTS * TILE, OFF_BAR = OFF_OUT + 8 * 4096, OFF_CUR = OFF_BAR + 24 * SLOTS + 96, SMEM = OFF_CUR + 8 * sizeof(Cursor);
 };
 
 __device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&v)[16]) {
@@ -231,13 +232,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_attn_prefill_kernel(const
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u, kv0 = smem0 + S::OFF_KV;
     const uint32_t full0 = smem0 + S::OFF_BAR, empty0 = full0 + 8 * S::SLOTS, clean0 = empty0 + 8 * S::SLOTS, qfull = clean0 + 8 * S::SLOTS, qempty = qfull + 8, sfull0 = qfull + 16,
-                   pfull0 = qfull + 32, phalf0 = qfull + 48, tmem_slot = qfull + 64;      // pfull, phalf: the weights of a tile's first and second 64 keys
+                   pfull0 = qfull + 32, phalf0 = qfull + 48, ofull0 = qfull + 64, tmem_slot = qfull + 80;      // pfull, phalf: the weights of a tile's first and second 64 keys
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int qrows = qtoks * p.group, block = 2 * qrows;                    // rows of a query tile, of a row block
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::SLOTS; ++s) mbar_init_a(full0 + 8 * s, 1), mbar_init_a(empty0 + 8 * s, 1), mbar_init_a(clean0 + 8 * s, 1);
         mbar_init_a(qfull, 1), mbar_init_a(qempty, 1);
-        for (int w = 0; w < 2; ++w) mbar_init_a(sfull0 + 8 * w, 1), mbar_init_a(pfull0 + 8 * w, 4), mbar_init_a(phalf0 + 8 * w, 4);
+        for (int w = 0; w < 2; ++w) mbar_init_a(sfull0 + 8 * w, 1), mbar_init_a(pfull0 + 8 * w, 4), mbar_init_a(phalf0 + 8 * w, 4), mbar_init_a(ofull0 + 8 * w, 1);
         mbar_fence_init();
         prefetch_tmap(&map_q), prefetch_tmap(&map_k), prefetch_tmap(&map_v);
     }
@@ -364,7 +365,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_attn_prefill_kernel(const
                     if (lead && ok) {
                         values(0, sv, 1, acc);
                         if (more) scores(0, sk);
-                        umma_commit(sfull0);                                 // S0 of the next tile is there, O0 of this one too
+                        umma_commit(more ? sfull0 : ofull0);                 // S0 of the next tile is there, O0 of this one too
                     }
                     __syncwarp();
                     if (two) {
@@ -380,7 +381,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_attn_prefill_kernel(const
                         if (two) values(1, sv, 1, acc);
                         umma_commit(empty0 + 8 * sv);
                         if (two && more) scores(1, sk);
-                        if (two) umma_commit(sfull0 + 8);
+                        if (two) umma_commit((more ? sfull0 : ofull0) + 8);
                         if (more) umma_commit(empty0 + 8 * sk);
                         if (i + 2 == run) umma_commit(qempty);
                     }
@@ -420,12 +421,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_attn_prefill_kernel(const
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         // ---- softmax: one row a thread
         const int w = warp >> 2, rl = (warp & 3) * 32 + lane;
-        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lane_base + 128u * w, to = ts + 256u, sfull = sfull0 + 8 * w, pfull = pfull0 + 8 * w, phalf = phalf0 + 8 * w;
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lane_base + 128u * w, to = ts + 256u, sfull = sfull0 + 8 * w, ofull = ofull0 + 8 * w, pfull = pfull0 + 8 * w, phalf = phalf0 + 8 * w;
         const uint32_t stage = smem0 + S::OFF_OUT + warp * 4096;             // 32 rows x 128 bytes on their way to memory
         const float scale2 = fabsf(p.scale2);
         const uint64_t scale_pair = pair_of(scale2, scale2);
         const bool flip = p.scale2 < 0.f;
-        uint32_t sparity = 0;
+        uint32_t sparity = 0, oparity = 0;
         int flags = 0;
         // the warp's place in its run lies in shared memory: a row's 128 scores take the registers
         Cursor& c = *reinterpret_cast<Cursor*>(smem_raw + (smem0 - smem_u32(smem_raw)) + S::OFF_CUR + warp * sizeof(Cursor));
@@ -540,8 +541,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_attn_prefill_kernel(const
                     split_pair(add_pair(sum[0], sum[1]), a, b);
                     l += a + b;
                 }
-                if (!failed && !wait_here(sfull, sparity)) failed = true;    // the last O
-                sparity ^= 1u;
+                if (!failed && !wait_here(ofull, oparity)) failed = true;    // the last O
+                oparity ^= 1u;
                 tc_fence_after();
                 // ---- output: 128 bytes of each of the warp's rows at a time through shared memory (16-byte pieces, swizzled), so that eight lanes store one row's
                 const bool whole = from == 0 && run == c.s.n;
