@@ -288,7 +288,7 @@ int kyb_rope_append(const kyb_rope_append_args* args, void* stream);
  * [cu_q[0], cu_q[batch]) stay as they are; out may be q. max_q: the largest number of rows of a request (it chooses the kernel; rows of longer requests are served too).
  * Table entries outside [0, pages) read as tokens of zeros; entries and cache places behind a request's last token, and those in front of the window of its first row,
  * may hold anything. Other places must hold finite values. Scores, sums and the output's accumulation in 32 bits; the weights enter the product with V in the
- * inputs' type, as the tensor cores take them. Scratch: kyb_paged_attention_workspace_bytes, private to the call until it has run. */
+ * inputs' type, as the tensor cores take them (fp16: what lies under 2^-32 of a row's largest weight is lost). Scratch: kyb_paged_attention_workspace_bytes, private to the call until it has run. */
 size_t kyb_paged_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t max_q, int64_t cols, int page, int hq, int hkv, int d);
 typedef struct {
     const void *q, *k_cache, *v_cache, *table, *kv_lens, *cu_q;

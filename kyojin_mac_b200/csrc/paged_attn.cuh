@@ -32,6 +32,14 @@ struct AttnParams {
 // flags of a CTA's note: its first run continues an item (and ends it), its last run begins an item that the next CTA continues
 constexpr int NOTE_CONTINUES = 1, NOTE_ENDS = 2, NOTE_BEGINS = 4;
 
+// A row's weights are 2^(below + score - m), rounded to the inputs' type for the product with V; the reference m is the largest score when it is set and moves when a score
+// passes it by `move`. The factor 2^below is in all parts of a row alike and leaves with the division by their sum. It is there for fp16, which has steps of 2^-24: under a
+// largest weight of 1, those below 2^-25 would be gone, and where one key takes nearly all of the mass (a first token, say) the many small ones add up to something all the
+// same. With the largest between 2^7 and 2^15 what is lost is 2^-32 of it. (2^15 keeps fp16 finite; the sums are in 32 bits. A smaller `move` would leave room for a larger
+// factor, but scores pass the first tile's largest by 2^4 now and then, by 2^8 hardly ever.) bf16 has the exponents of 32 bits and needs no factor.
+template <typename T> struct Weights { static constexpr float below = 7.f, move = 8.f; };
+template <> struct Weights<__nv_bfloat16> { static constexpr float below = 0.f, move = 15.f; };
+
 #ifdef __CUDACC__
 // The keys that a block of rows sees: tiles of `tile` keys, first those of the sinks, then those of the window (or of the whole context).
 struct KeySpan {

@@ -4,7 +4,7 @@
 // bytes, the pieces lie anywhere). A consumer warp owns 16 keys of every stage and everything about them, so the loop has no barrier among warps: with
 // mma.m16n8k16 it forms S^T = K Q^T (keys on the M side: 8 rows fill the N side, no padding up to G = 8), keeps its own reference maximum and sum per row, turns the
 // weights around in registers (movmatrix) and accumulates O^T = V^T P^T. tcgen05 would compute 128 rows for 8; here the tensor work is a sixth of the time the bytes take.
-// The reference maximum of a row moves only when a score passes it by 2^8 (a warp vote), so the usual stage needs no shuffle and no rescaling.
+// The reference maximum of a row moves only when a score passes it by 2^8 (bf16: 2^15; a warp vote), so the usual stage needs no shuffle and no rescaling.
 // Measured, 64 / 8 heads of 128: 64 sequences of 1000 to 16000 tokens 329 us = 6.7 TB/s, one of 778 tokens 9.8 us (both launches); counters: DRAM 1.01 x the necessary bytes,
 // issue slots 17 %. Requests of up to 16 rows come here, since their loop needs no more than the bytes' time; with 32 rows (four tokens of 8 heads, 8000 cached) the prefill
 // kernel takes 368 us for 64 requests, where the bytes take 320, and this one would read the keys again for every 16 rows.
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(DC_THREADS, 2) paged_attn_decode_kernel(const 
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) over |= fmaxf(x[n][e], x[n][2 + e]) > m[n][e] + 8.f;
+                    for (int e = 0; e < 2; ++e) over |= fmaxf(x[n][e], x[n][2 + e]) > m[n][e] + Weights<T>::move;
                 if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(DC_THREADS, 2) paged_attn_decode_kernel(const 
                 uint32_t pf[NT][2];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+                    const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0] - Weights<T>::below, m1 = m[n][1] == -INFINITY ? 0.f : m[n][1] - Weights<T>::below;
                     const float a = exp2_fast(x[n][0] - m0), b = exp2_fast(x[n][1] - m1), u = exp2_fast(x[n][2] - m0), w = exp2_fast(x[n][3] - m1);
                     l[n][0] += a + u, l[n][1] += b + w;
                     pf[n][0] = turn8x8(pack2<T>(a, b)), pf[n][1] = turn8x8(pack2<T>(u, w));

@@ -10,7 +10,7 @@
 // with one query tile while the softmax of the other runs; S(j+1) may overwrite P(j) without a wait in between, since one thread issues both products to the SM's one tensor
 // core, which runs them in that order. An item's last O has a barrier of its own: on the scores' one the next item's first scores, which wait for nothing of the softmax, could end
 // a second phase before a late softmax warp has seen the first, and a wait by parity would not pass any more. A row's reference maximum moves only when a score passes it by
-// 2^15, so O is rescaled (by the softmax warps themselves, in tensor memory) hardly ever; sums are of the unrounded weights, in 32 bits.
+// 2^8 (bf16: 2^15), so O is rescaled (by the softmax warps themselves, in tensor memory) hardly ever; sums are of the unrounded weights, in 32 bits.
 // Measured, 64 / 8 heads of 128: 1024 tokens on 8192 cached ones 245 to 250 us, a prompt of 8192 tokens 910 us = 1210 TFLOP/s; 3200 clocks a pair of tiles, of which the tensor
 // cores and the special-function units are busy 2050 each.
 // Keys that a row does not see are masked by selection in the tiles at the borders; values in places that no row of the block sees are cleared in shared memory, since such
@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_attn_prefill_kernel(const
                     // weights of 32 keys to tensor memory, their sum added to `sum`
                     uint64_t m_pair, sum[2];
                     auto reference = [&]() {
-                        const float m0 = m == -INFINITY ? 0.f : -m;
+                        const float m0 = m == -INFINITY ? 0.f : Weights<T>::below - m;
                         m_pair = pair_of(m0, m0), sum[0] = sum[1] = 0;
                     };
                     float t[4];
@@ -496,7 +496,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_attn_prefill_kernel(const
                         tmem_st_16(ts + 16 * q, pk);
                     };
                     // With heads of 64 the first half's weights are made with the reference as it is while the maximum is found, and again in the rare tile where a score
-                    // passes the reference by 2^15, beyond which fp16 would overflow: 219 -> 208 us for 1024 tokens on 8192. With heads of 128, where the wait for the
+                    // passes the reference too far: 219 -> 208 us for 1024 tokens on 8192. With heads of 128, where the wait for the
                     // products is the longer part, it gained nothing (252 -> 255 us): there, as in the first tile of an item, the maximum comes first.
                     if (D == 64 && i) {
                         reference();
@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_attn_prefill_kernel(const
                             for (int e = 2; e < 32; e += 2) t[q] = max3(t[q], __uint_as_float(v[q][e]), __uint_as_float(v[q][e + 1]));
                     }
                     const float top = fmaxf(max3(t[0], t[1], t[2]), t[3]) * scale2;
-                    const bool over = top > m + 15.f;                        // false where nothing is seen yet (-inf on both sides)
+                    const bool over = top > m + Weights<T>::move;            // false where nothing is seen yet (-inf on both sides)
                     const bool move = __any_sync(0xffffffffu, over);
                     if (move || D != 64 || i == 0) {
                         const float f = !over ? 1.f : m == -INFINITY ? 0.f : exp2_fast(m - top);

@@ -37,3 +37,32 @@ def test_short_items_follow_each_other(hq, hkv, d, lo, hi):
     ops.check_device_status()
     want, tol = R.attention(q, k, v, table, lens, cu, d ** -0.5, 0, 0)
     assert ((first.cpu().double() - want).abs() <= tol).all()
+
+
+# ------------------------------------------------------------------------------------------------ a dominant key
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("d,qn,n,b", [(128, 1, 9000, 1), (64, 2, 5000, 300), (128, 4, 3500, 300), (128, 70, 6001, 1), (64, 300, 4100, 1)])
+@pytest.mark.parametrize("at", [0, 3000])
+@pytest.mark.parametrize("above", [18.0, 22.0, 25.5, 27.0])
+def test_dominant_key(above, at, d, qn, n, b, dt):
+    """One key takes nearly all of the mass (its score 2^above over the others' level), its value is a thousandth of theirs: what the many others add up to shows in the output.
+    A weight is rounded relative to a reference that lies 2^7 at least under the row's largest, so fp16 loses 2^-32 of the largest weight per key at most, not 2^-25: the bound of
+    `R.attention` with its term for that taken 2^-7 times. b requests share the pages, so that one CTA walks a whole context."""
+    g = torch.Generator().manual_seed(int(above) + d)
+    k, v, table = R.pool([n], 64, 1, d, torch.float32, 41, device="cpu")
+    k = torch.where(torch.isnan(k), k, torch.randn(k.shape, generator=g) * 0.05)
+    k[..., 0] = torch.where(torch.isnan(k[..., 0]), k[..., 0], 0.0)
+    v = torch.where(torch.isnan(v), v, 1.0 + 0.25 * torch.rand(v.shape, generator=g))
+    page, place = int(table[0, at // 64]), at % 64
+    k[page, 0, place] = 0.0
+    k[page, 0, place, 0], v[page, 0, place] = above * 0.6931 * d ** 0.5 / 16.0, 0.001
+    q = torch.randn((qn, 4, d), generator=g) * 0.5
+    q[..., 0] = 16.0
+    q, k, v, table = q.to(dt).cuda(), k.to(dt).cuda(), v.to(dt).cuda(), table.cuda()
+    got = ops.paged_attention(q.repeat(b, 1, 1), k, v, table.repeat(b, 1), _i32([n] * b), _offsets([qn] * b), qn).view(b, qn, 4, d)
+    want, tol = R.attention(q, k, v, table, _i32([n]), _i32([0, qn]), d ** -0.5, 0, 0)
+    if dt == F16:
+        keys = (torch.arange(n - qn, n) + 1.0).double()[:, None, None]
+        tol = tol - keys * 2.0 ** -25 * (1 - 2.0 ** -7) * float(v[~v.isnan()].abs().max())
+    err = (got.cpu().double() - want).abs()
+    assert (tol > 0).all() and (err <= tol).all(), float((err / tol).max())
