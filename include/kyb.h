@@ -286,6 +286,8 @@ int kyb_rope_append(const kyb_rope_append_args* args, void* stream);
 /* attention of a step's new tokens over the cache: request r owns the rows [cu_q[r], cu_q[r + 1]) of q and out ([tokens][hq][d]), its last row is its token
  * kv_lens[r] - 1. The token at position p sees key j when j <= p and, with window > 0, j > p - window or j < sinks. A row that sees nothing gives zeros; rows outside
  * [cu_q[0], cu_q[batch]) stay as they are; out may be q. max_q: the largest number of rows of a request (it chooses the kernel; rows of longer requests are served too).
+ * The offsets do not fall. Where they do, a row that two requests share takes the result of either; where the requests would own more rows than there are, nothing is written and the
+ * device status word says so (KYB_EINVAL from kyb_check_device_status).
  * Table entries outside [0, pages) read as tokens of zeros; entries and cache places behind a request's last token, and those in front of the window of its first row,
  * may hold anything. Other places must hold finite values. Scores, sums and the output's accumulation in 32 bits; the weights enter the product with V in the
  * inputs' type, as the tensor cores take them (fp16: what lies under 2^-32 of a row's largest weight is lost). Scratch: kyb_paged_attention_workspace_bytes, private to the call until it has run. */
@@ -306,7 +308,8 @@ int kyb_gemv_plan(int fmt, int64_t n, int64_t k, int64_t m, int* out8);
 /* the same for a caller that brings workspace_bytes of scratch (kyb_gemv_t16: another form where the best one needs more; 0 warps: none fits) */
 int kyb_gemv_plan_within(int fmt, int64_t n, int64_t k, int64_t m, size_t workspace_bytes, int* out8);
 
-/* device status word of the calling thread's current device: nonzero after a bounded wait expired inside a kernel.
+/* device status word of the calling thread's current device: nonzero after a bounded wait expired inside a kernel (or
+ * after attention was given offsets that it cannot follow).
  * kyb_check_device_status synchronises `stream`, reads and clears it. */
 int kyb_check_device_status(void* stream);
 

@@ -77,6 +77,10 @@ int kyb_check_device_status(void* stream) {
     KYB_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
     if (v) {
         KYB_CUDA(cudaMemsetAsync(w, 0, sizeof(v), (cudaStream_t)stream));
+        if (v == KYB_DEV_ROWS_ATTN) {
+            kyb_set_error("device status 0x%x: attention was given offsets (cu_q) that fall, so that the requests own more rows than there are; nothing was written", v);
+            return KYB_EINVAL;
+        }
         kyb_set_error("device status 0x%x: a kernel gave up a bounded wait", v);
         return KYB_ETIMEOUT;
     }

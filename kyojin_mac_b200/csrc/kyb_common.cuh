@@ -62,6 +62,8 @@ __host__ __device__ constexpr bool kyb_has_mins16(int fmt) { return fmt == KYB_F
 #define KYB_DEV_TIMEOUT_GEMM 0x1002u
 #define KYB_DEV_TIMEOUT_ATTN 0x1003u
 #define KYB_DEV_TIMEOUT_SELFTEST 0x10FFu
+// and by kernels that found something in device memory that they cannot work with
+#define KYB_DEV_ROWS_ATTN 0x2001u
 
 #ifdef __CUDACC__
 // ------------------------------------------------------------------------------------------------ device side

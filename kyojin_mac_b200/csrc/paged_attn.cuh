@@ -71,6 +71,23 @@ __device__ __forceinline__ int request_rows(const AttnParams& p, int r, int& bas
     base = min(max(p.cu_q[r], 0), p.tokens);
     return min(max(p.cu_q[r + 1], base), p.tokens) - base;
 }
+// Whether a request's offsets fall. Where none do, the requests own no more rows than there are, and the host's bound of the units (fewer than 2^31 in all) rests on that.
+__device__ __forceinline__ bool offsets_fall(const AttnParams& p, int r) { return max(p.cu_q[r + 1], 0) < min(max(p.cu_q[r], 0), p.tokens); }
+// Where some do (0, T, 0, T, ... would give every second request all rows): whether the requests together still own no more than there are. If not, the sums of units could pass
+// 32 bits and the runs be anything, so nothing is done and the status word says why. All threads of the block call it; `sum` is a word of shared memory.
+__device__ __forceinline__ bool rows_hold(const AttnParams& p, unsigned long long* sum) {
+    __syncthreads();
+    if (threadIdx.x == 0) {                                                  // one thread: a shared sum here cost the prefill kernel for heads of 64 1 % (206 -> 208 us) by its softmax loop's code
+        int base;
+        *sum = 0;
+#pragma unroll 1
+        for (int r = 0; r < p.batch; ++r) *sum += (unsigned)request_rows(p, r, base);
+    }
+    __syncthreads();
+    if (*sum <= (unsigned long long)p.tokens) return true;
+    if (blockIdx.x == 0 && threadIdx.x == 0) atomicExch(p.status, KYB_DEV_ROWS_ATTN);
+    return false;
+}
 __device__ __forceinline__ int request_keys(const AttnParams& p, int r) { return min(max(p.kv_lens[r], 0), 1 << 30); }
 __device__ __forceinline__ int row_blocks(const AttnParams& p, int tokens, int block) { return (tokens * p.group + block - 1) / block; }
 
@@ -99,7 +116,7 @@ struct Runs {
     static __device__ __forceinline__ int cost(int at, int taken) { return taken + (at ? 0 : OVER); }
 };
 
-// border c of `runs` equal runs over `total` units (fewer than 2^31, the host sees to it)
+// border c of `runs` equal runs over `total` units (fewer than 2^31: the host sees to it for requests side by side, rows_hold to those)
 __device__ __forceinline__ int run_border(int total, int runs, int c) {
     const int each = total / runs;
     return each * c + min(c, total - each * runs);

@@ -54,15 +54,24 @@ __device__ __forceinline__ int request_units(const AttnParams& p, int r, int blo
 }
 
 // First item and length of this CTA's run: every thread of the block takes part; the result is in *out (shared).
-__device__ __forceinline__ void find_run(const AttnParams& p, int block, Cursor* out, int* sums, int threads) {
+__device__ __forceinline__ void find_run(const AttnParams& p, int block, Cursor* out, int* sums, unsigned long long* rows, int threads) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = threads / 32;
-    int mine = 0;
-    for (int r = tid; r < p.batch; r += threads) mine += request_units(p, r, block);
-    const int first = mine;                                                 // (this thread's only request when there are no more of them than threads)
+    unsigned mine = 0, seen = 0;
+    bool falls = false;
+    for (int r = tid; r < p.batch; r += threads) {
+        int base;
+        seen += (unsigned)request_rows(p, r, base), falls |= offsets_fall(p, r);
+        if (seen > (unsigned)p.tokens) {                                    // (the sum over a request's blocks is a loop: it ends here where offsets fall)
+            falls = true;
+            break;
+        }
+        mine += (unsigned)request_units(p, r, block);
+    }
+    const int first = (int)mine;                                            // (this thread's only request when there are no more of them than threads)
     mine = __reduce_add_sync(0xffffffffu, mine);
-    if (lane == 0) sums[warp] = mine;
+    if (lane == 0) sums[warp] = (int)mine;
     if (tid == 0) out->left = 0;
-    __syncthreads();
+    if (__syncthreads_or(falls) && !rows_hold(p, rows)) return;
     int total = 0;
     for (int w = 0; w < warps; ++w) total += sums[w];
     const int ctas = min((int)gridDim.x, total), c = blockIdx.x;
@@ -109,6 +118,7 @@ __global__ void __launch_bounds__(DC_THREADS, 2) paged_attn_decode_kernel(const 
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ Cursor start;
     __shared__ int sums[DC_WARPS + 1];
+    __shared__ unsigned long long rows;
     const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* const smem_g = smem_raw + (smem0 - smem_u32(smem_raw));
     const uint32_t full0 = smem0 + S::OFF_BAR, empty0 = full0 + 8 * S::STAGES;
@@ -120,7 +130,7 @@ __global__ void __launch_bounds__(DC_THREADS, 2) paged_attn_decode_kernel(const 
         prefetch_tmap(&map_v);
     }
     pdl_wait();                                                              // what is above runs while the kernel before drains
-    find_run(p, S::ROWS, &start, sums, DC_THREADS);
+    find_run(p, S::ROWS, &start, sums, &rows, DC_THREADS);
     Cursor c = start;
     pdl_launch_dependents();
     const int page = 1 << p.page_log2, piece = min(page, DC_TILE), piece_log2 = min(p.page_log2, 6), pieces = DC_TILE >> piece_log2;

@@ -85,6 +85,7 @@ __device__ __forceinline__ int first_end_above(const int* v, int n, int x) {
 }
 
 struct RunFinder {
+    unsigned long long rows;
     int tokens[PF_THREADS], kv[PF_THREADS], blocks_end[PF_THREADS], units[PF_THREADS], sums[2][PF_THREADS / 32];
     Cursor run;
     int at, request;
@@ -107,25 +108,27 @@ __device__ __forceinline__ int scan_block(int v, int* sums, int& total) {
     }
     return v;
 }
-// rows, keys and (scanned) row blocks of up to PF_THREADS requests from r0 on; gives the number of their row blocks
+// rows, keys and (scanned) row blocks of up to PF_THREADS requests from r0 on, for all threads; gives the number of their row blocks (-1: the requests own more rows than there are)
 __device__ __forceinline__ int load_chunk(const AttnParams& p, int block, int r0, RunFinder& f) {
     const int tid = threadIdx.x, n = min(PF_THREADS, p.batch - r0);
     int nb = 0;
+    bool falls = false;
     if (tid < n) {
+        falls = offsets_fall(p, r0 + tid);
         int base;
         f.tokens[tid] = request_rows(p, r0 + tid, base), f.kv[tid] = request_keys(p, r0 + tid);
         nb = row_blocks(p, f.tokens[tid], block);
     }
     int all;
     f.blocks_end[tid] = scan_block(nb, f.sums[0], all);
-    return all;
+    return __syncthreads_or(falls) && !rows_hold(p, &f.rows) ? -1 : all;
 }
-// their units, of all heads: the row blocks of all of them are shared among the threads
+// their units, of all heads: the row blocks of all of them are shared among the threads (-1 as above)
 __device__ __forceinline__ int count_chunk(const AttnParams& p, int block, int r0, RunFinder& f, int& end) {
     const int tid = threadIdx.x, n = min(PF_THREADS, p.batch - r0);
     f.units[tid] = 0;
     const int all = load_chunk(p, block, r0, f);
-    __syncthreads();
+    if (all < 0) return -1;
     for (int i0 = tid & ~31; i0 < all; i0 += PF_THREADS) {                   // whole numbers: the order of the additions does not matter
         const int i = min(i0 + (tid & 31), all - 1), r = first_end_above(f.blocks_end, n, i), rb = i - (r ? f.blocks_end[r - 1] : 0);
         const int u = i0 + (tid & 31) < all ? PrefillRuns::units(key_span(p, f.tokens[r], f.kv[r], block, rb, PF_TILE)) * p.hkv : 0;
@@ -156,7 +159,7 @@ __device__ __forceinline__ void find_run_wide(const AttnParams& p, int block, Ru
     if (tid == 0) f.run.left = 0, f.request = 0, f.at = 0;
     if (FEW && p.batch <= PF_THREADS) {
         const int all = load_chunk(p, block, 0, f);
-        __syncthreads();
+        if (all < 0) return;
         if (all <= PF_THREADS) {                                             // a row block a thread: one more scan gives the sums and the place
             const int r = tid < all ? first_end_above(f.blocks_end, p.batch, tid) : 0, rb = tid - (r ? f.blocks_end[r - 1] : 0);
             const int one = tid < all ? PrefillRuns::units(key_span(p, f.tokens[r], f.kv[r], block, rb, PF_TILE)) : 0, n = one * p.hkv;
@@ -173,6 +176,7 @@ __device__ __forceinline__ void find_run_wide(const AttnParams& p, int block, Ru
     for (int r0 = 0; r0 < p.batch; r0 += PF_THREADS) {
         if (r0) __syncthreads();
         mine = count_chunk(p, block, r0, f, end), total += mine;
+        if (mine < 0) return;
     }
     const int ctas = min((int)gridDim.x, total);
     const int u0 = c < ctas ? run_border(total, ctas, c) : 0, u1 = c < ctas ? run_border(total, ctas, c + 1) : 0;

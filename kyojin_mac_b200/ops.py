@@ -756,6 +756,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     window: int = 0, sinks: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of a step's new tokens over a paged cache: q fp16 / bf16 [T, heads, d] packed by request (rows [cu_q[r], cu_q[r + 1]); the last one is token
     kv_lens[r] - 1), keys and values through the block table [batch, columns]. Causal; window > 0: the last `window` tokens only, and the first `sinks` ones.
+    cu_q does not fall: where it does so far that the requests would own more than T rows, nothing is written and `check_device_status` raises.
     max_q: the largest number of new tokens of a request (chooses the kernel; requests with more are served all the same). scale: d ** -0.5 unless given.
     A row that sees nothing (kv_lens 0) gives zeros; rows behind the last request are left as they were (undefined without `out`). `out` may be q itself. Returns out [T, heads, d]."""
     dev = q.get_device()

@@ -6,6 +6,7 @@ import torch
 
 import paged_reference as R
 from kyojin_mac_b200 import ops
+from kyojin_mac_b200._lib import EINVAL, KybError
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +67,33 @@ def test_dominant_key(above, at, d, qn, n, b, dt):
         tol = tol - keys * 2.0 ** -25 * (1 - 2.0 ** -7) * float(v[~v.isnan()].abs().max())
     err = (got.cpu().double() - want).abs()
     assert (tol > 0).all() and (err <= tol).all(), float((err / tol).max())
+
+
+# ------------------------------------------------------------------------------------------------ offsets that give the requests more rows than there are
+@pytest.mark.parametrize("rows,pairs,max_q,hkv,cols", [(64, 20, 1, 2, 4), (64, 20, 64, 2, 4), (5, 300, 1, 1, 4), (20000, 2000, 1, 1, 300), (20000, 2000, 300, 1, 300), (30, 1, 30, 1, 4)])
+def test_offsets_that_overlap(rows, pairs, max_q, hkv, cols):
+    """Offsets 0, T, 0, T, ...: every second request would own all rows, and the sums of their key tiles could pass any bound. Nothing is written, the status word tells; calls
+    with good offsets are served before and after."""
+    page, d = 64, 64
+    k, v = (torch.randn((3, hkv, page, d), device="cuda").to(F16) for _ in range(2))
+    q = torch.randn((rows, 4 * hkv, d), device="cuda").to(F16)
+    batch = 2 * pairs + 1
+    table = torch.zeros((batch, cols), dtype=torch.int32, device="cuda")
+    lens = torch.full((batch,), page, dtype=torch.int32, device="cuda")
+    good = torch.full((batch + 1,), rows, dtype=torch.int32, device="cuda")
+    good[0] = 0
+    bad = torch.zeros_like(good)
+    bad[1::2] = rows
+    lens[0] = max(page, rows)
+    want = ops.paged_attention(q, k, v, table, lens, good, max_q)
+    out = torch.full_like(q, 6.0)
+    lens[:] = cols * page
+    ops.paged_attention(q, k, v, table, lens, bad, max_q, out=out)
+    with pytest.raises(KybError, match="offsets") as e:
+        ops.check_device_status()
+    assert e.value.status == EINVAL
+    assert (out == 6.0).all()
+    lens[:] = page
+    lens[0] = max(page, rows)
+    assert torch.equal(ops.paged_attention(q, k, v, table, lens, good, max_q, out=out), want)
+    ops.check_device_status()
