@@ -271,7 +271,7 @@ int kyb_paged_step(const kyb_paged_step_args* args, void* stream);
 int kyb_paged_release(void* lens, const void* which, void* table, int64_t ld_table, int64_t batch, int64_t cols, int page, void* free_pages, int64_t free_cap,
                       void* free_count, void* refused, void* stream);
 /* rotary positions and cache append: the pairs of the first rot values of every query and key head (interleaved: (2 i, 2 i + 1), else (i, i + rot / 2)) turned by
- * positions[t] * inv_freq[i] (fp32 [rot / 2]; product and reduction in 64 bits) and scaled by mscale; queries to q_out (may be q), keys and values to the cache at
+ * positions[t] * inv_freq[i] (fp32 [rot / 2]; product and reduction in 64 bits) and scaled by mscale; queries to q_out (q itself, or memory apart from the rest), keys and values to the cache at
  * slots[t]. A row with positions[t] < 0 is left alone, a slot outside the cache stores nothing. hkv = 0: queries only. d a multiple of 8 up to 256, rot a
  * multiple of 16. Strides in elements. A slot that two rows share holds values of either. */
 typedef struct {
@@ -285,7 +285,7 @@ typedef struct {
 int kyb_rope_append(const kyb_rope_append_args* args, void* stream);
 /* attention of a step's new tokens over the cache: request r owns the rows [cu_q[r], cu_q[r + 1]) of q and out ([tokens][hq][d]), its last row is its token
  * kv_lens[r] - 1. The token at position p sees key j when j <= p and, with window > 0, j > p - window or j < sinks. A row that sees nothing gives zeros; rows outside
- * [cu_q[0], cu_q[batch]) stay as they are; out may be q. max_q: the largest number of rows of a request (it chooses the kernel; rows of longer requests are served too).
+ * [cu_q[0], cu_q[batch]) stay as they are; out is q itself, or memory apart from q and the cache. max_q: the largest number of rows of a request (it chooses the kernel; rows of longer requests are served too).
  * The offsets do not fall. Where they do, a row that two requests share takes the result of either; where the requests would own more rows than there are, nothing is written and the
  * device status word says so (KYB_EINVAL from kyb_check_device_status).
  * Table entries outside [0, pages) read as tokens of zeros; entries and cache places behind a request's last token, and those in front of the window of its first row,

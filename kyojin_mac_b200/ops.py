@@ -547,6 +547,49 @@ def _cache(t, name, like=None):
         raise ValueError(f"{name}: the tokens of a page and head must be dense, strides multiples of 8 elements, the start 16-byte aligned; got strides {t.stride()}")
 
 
+class _Views:
+    """Where the tensors of a call lie relative to each other: what a call writes overlaps nothing else of it, or other blocks of the launch would read values that this one has
+    written already. views: (name, tensor) of 16-bit tensors that come as addresses later; writes: names of those written; same: a pair that may be one and the same memory."""
+
+    def __init__(self, views, writes, same):
+        self.names = [n for n, _ in views]
+        self.dims = [sorted(((s, n) for n, s in zip(t.shape, t.stride()) if n > 1), reverse=True) for _, t in views]
+        size = [2 * self.extent(d) if t.numel() else 0 for d, (_, t) in zip(self.dims, views)]
+        self.pairs = [(i, j, size[i], size[j], {a, b} == set(same) and self.dims[i] == self.dims[j]) for j, b in enumerate(self.names) for i, a in enumerate(self.names[:j])
+                      if a in writes or b in writes]
+        self.passed = set()                                                  # offsets of the tensors from the first that have passed
+
+    @staticmethod
+    def extent(dims):
+        return sum(s * (n - 1) for s, n in dims) + 1
+
+    @classmethod
+    def disjoint(cls, a, b, offset):
+        """Whether views of the dims a, b = [(stride, size), ...] (falling strides, in elements), the second starting `offset` elements behind the first, are certain to share nothing: their
+        ranges lie apart, or they have outer strides in common and lie apart within those (q and k of one q | k | v product)."""
+        if offset >= cls.extent(a) or -offset >= cls.extent(b):
+            return True
+        outer = 0
+        while a and b and a[0][0] == b[0][0] > 1 and outer % a[0][0] == 0:
+            outer, a, b = a[0][0], a[1:], b[1:]
+            if offset % outer >= cls.extent(a) and offset % outer + cls.extent(b) <= outer:
+                return True
+        return False
+
+    def check(self, first, *others):
+        offsets = tuple([p - first for p in others])
+        if offsets in self.passed:
+            return
+        ptrs = (0,) + offsets
+        for i, j, m, n, same in self.pairs:
+            off = ptrs[j] - ptrs[i]
+            if -n < off < m and not (same and off == 0) and (off % 2 or not self.disjoint(self.dims[i], self.dims[j], off // 2)):
+                raise ValueError(f"{self.names[i]} and {self.names[j]} overlap in memory")
+        if len(self.passed) >= 256:
+            self.passed.clear()
+        self.passed.add(offsets)
+
+
 # Calls whose shapes, strides, types and numbers have passed the checks (their description; nothing of their data): a decode step repeats its calls for every layer and
 # token, and the checks cost more than the launch.
 _passed: dict = {}
@@ -680,8 +723,9 @@ def _rope_check(key, q, k, v, positions, slots, inv_freq, kc, vc, interleaved, m
         ks, vs, kcs, vcs = k.stride()[:2], v.stride()[:2], kc.stride()[:2], vc.stride()[:2]
         pages, hkv, page = kc.shape[:3]
     os_ = (hq * d, d) if out is None else out.stride()[:2]
-    return _remember(key, _lib.ROPE_APPEND_SPLIT[1].pack(*q.stride()[:2], *ks, *vs, *os_, *kcs, *vcs, T, hq, hkv, d, 2 * inv_freq.shape[0], 1 if interleaved else 0, _DT[q.dtype], pages, page,
-                                                         mscale))
+    views = [(n, t) for n, t in (("q", q), ("k", k), ("v", v), ("k_cache", kc), ("v_cache", vc), ("out", out)) if t is not None]
+    return _remember(key, (_lib.ROPE_APPEND_SPLIT[1].pack(*q.stride()[:2], *ks, *vs, *os_, *kcs, *vcs, T, hq, hkv, d, 2 * inv_freq.shape[0], 1 if interleaved else 0, _DT[q.dtype], pages, page,
+                                                          mscale), _Views(views, [n for n, _ in views if n in ("k_cache", "v_cache", "out")], ("q", "out"))))
 
 
 def _rope_call(q, k, v, positions, slots, inv_freq, kc, vc, interleaved, mscale, out):
@@ -697,19 +741,28 @@ def _rope_call(q, k, v, positions, slots, inv_freq, kc, vc, interleaved, mscale,
                v.get_device(), positions.get_device(), slots.get_device(), inv_freq.get_device(), kc.get_device(), vc.get_device(), interleaved, mscale)
     if out is not None:
         key += (out.shape, out.stride(), out.dtype, out.get_device())
-    numbers = None if grad or not inv_freq.is_contiguous() else _passed.get(key)
-    if numbers is None:
-        numbers = _rope_check(key, q, k, v, positions, slots, inv_freq, kc, vc, interleaved, mscale, out)
+    known = None if grad or not inv_freq.is_contiguous() else _passed.get(key)
+    if known is None:
+        known = _rope_check(key, q, k, v, positions, slots, inv_freq, kc, vc, interleaved, mscale, out)
     if dev != torch.cuda.current_device() if _cur_device is None else dev != _cur_device():
         with torch.cuda.device(dev):
             return _rope_call(q, k, v, positions, slots, inv_freq, kc, vc, interleaved, mscale, out)
-    if out is None:
+    numbers, views = known
+    given = out is not None
+    if not given:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     qp, pp, ip, op = q.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), out.data_ptr()
     if k is None:
+        if given:
+            views.check(qp, op)
         ptrs = _lib.ROPE_APPEND_SPLIT[0].pack(qp, 0, 0, pp, 0, ip, op, 0, 0)
     else:
-        ptrs = _lib.ROPE_APPEND_SPLIT[0].pack(qp, k.data_ptr(), v.data_ptr(), pp, slots.data_ptr(), ip, op, kc.data_ptr(), vc.data_ptr())
+        kp, vp, kcp, vcp = k.data_ptr(), v.data_ptr(), kc.data_ptr(), vc.data_ptr()
+        if given:
+            views.check(qp, kp, vp, kcp, vcp, op)
+        else:
+            views.check(qp, kp, vp, kcp, vcp)
+        ptrs = _lib.ROPE_APPEND_SPLIT[0].pack(qp, kp, vp, pp, slots.data_ptr(), ip, op, kcp, vcp)
     rc = _lib.lib().kyb_rope_append(ptrs + numbers, _stream())
     if rc:
         _lib.check(rc)
@@ -718,14 +771,15 @@ def _rope_call(q, k, v, positions, slots, inv_freq, kc, vc, interleaved, mscale,
 
 def rope(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False, mscale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
     """x fp16 / bf16 [tokens, heads, d] with the first rot = 2 len(inv_freq) values of every head turned: pairs (i, i + rot / 2), or (2 i, 2 i + 1) when interleaved, by
-    positions[t] * inv_freq[i], scaled by mscale. Rows of a negative position are left as they are in `out` (which may be x, or memory apart from it)."""
+    positions[t] * inv_freq[i], scaled by mscale. Rows of a negative position are left as they are in `out` (x itself, or memory apart from it)."""
     return _rope_call(x, None, None, positions, None, inv_freq, None, None, interleaved, mscale, out)
 
 
 def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, inv_freq: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                 interleaved: bool = False, mscale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
     """`rope` of a step's queries, and in the same launch its keys (turned) and values into the cache [pages, kv heads, tokens of a page, d] at slots[t]. q [T, heads, d],
-    k and v [T, kv heads, d] may be views of one q | k | v product. Returns the turned queries. Rows with a negative position are left alone, a slot outside the cache
+    k and v [T, kv heads, d] may be views of one q | k | v product. Returns the turned queries (in `out`: q itself, or memory apart
+    from the other tensors). Rows with a negative position are left alone, a slot outside the cache
     stores nothing. The slots of a step are distinct (paged_step's are): one that two rows share holds values of either."""
     return _rope_call(q, k, v, positions, slots, inv_freq, k_cache, v_cache, interleaved, mscale, out)
 
@@ -748,7 +802,8 @@ def _attention_check(key, q, kc, vc, table, kv_lens, cu_q, max_q, scale, window,
     with torch.cuda.device(q.device):
         need = _lib.lib().kyb_paged_attention_workspace_bytes(b, T, max_q, cols, page, hq, hkv, d)
     os_ = (hq * d, d) if out is None else out.stride()[:2]
-    return _remember(key, (need, _lib.PAGED_ATTENTION_SPLIT[1].pack(*q.stride()[:2], *kc.stride()[:2], *vc.stride()[:2], *os_, pages, page, max(table.stride(0), cols), cols, b, T, max_q, hq, hkv,
+    views = None if out is None else _Views([("q", q), ("k_cache", kc), ("v_cache", vc), ("out", out)], ["out"], ("q", "out"))
+    return _remember(key, (need, views, _lib.PAGED_ATTENTION_SPLIT[1].pack(*q.stride()[:2], *kc.stride()[:2], *vc.stride()[:2], *os_, pages, page, max(table.stride(0), cols), cols, b, T, max_q, hq, hkv,
                                                                     d, _DT[q.dtype], window, sinks, need, d ** -0.5 if scale is None else scale)))
 
 
@@ -758,7 +813,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     kv_lens[r] - 1), keys and values through the block table [batch, columns]. Causal; window > 0: the last `window` tokens only, and the first `sinks` ones.
     cu_q does not fall: where it does so far that the requests would own more than T rows, nothing is written and `check_device_status` raises.
     max_q: the largest number of new tokens of a request (chooses the kernel; requests with more are served all the same). scale: d ** -0.5 unless given.
-    A row that sees nothing (kv_lens 0) gives zeros; rows behind the last request are left as they were (undefined without `out`). `out` may be q itself. Returns out [T, heads, d]."""
+    A row that sees nothing (kv_lens 0) gives zeros; rows behind the last request are left as they were (undefined without `out`). `out` is q itself
+    or memory apart from q and the cache. Returns out [T, heads, d]."""
     dev = q.get_device()
     key = (dev, q.shape, q.is_contiguous() or q.stride(), q.dtype, k_cache.shape, k_cache.is_contiguous() or k_cache.stride(), k_cache.dtype, v_cache.shape,
            v_cache.is_contiguous() or v_cache.stride(), v_cache.dtype, table.shape, table.is_contiguous() or table.stride(), table.dtype, kv_lens.shape, kv_lens.dtype, kv_lens.is_contiguous(),
@@ -770,12 +826,15 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if dev != torch.cuda.current_device() if _cur_device is None else dev != _cur_device():
         with torch.cuda.device(dev):
             return paged_attention(q, k_cache, v_cache, table, kv_lens, cu_q, max_q, scale, window, sinks, out)
-    need, numbers = known
+    need, views, numbers = known
+    qp, kp, vp = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
+        views.check(qp, kp, vp, out.data_ptr())
     # the call's own scratch: captured graphs that replay side by side share nothing, nor do calls of two threads on one stream, whose launches may interleave
     ws = q.new_empty((need + 1) // 2)
-    rc = _lib.lib().kyb_paged_attention(_lib.PAGED_ATTENTION_SPLIT[0].pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), kv_lens.data_ptr(), cu_q.data_ptr(),
+    rc = _lib.lib().kyb_paged_attention(_lib.PAGED_ATTENTION_SPLIT[0].pack(qp, kp, vp, table.data_ptr(), kv_lens.data_ptr(), cu_q.data_ptr(),
                                                                            out.data_ptr(), ws.data_ptr()) + numbers, _stream())
     if rc:
         _lib.check(rc)

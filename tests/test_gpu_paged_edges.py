@@ -97,3 +97,41 @@ def test_offsets_that_overlap(rows, pairs, max_q, hkv, cols):
     lens[0] = max(page, rows)
     assert torch.equal(ops.paged_attention(q, k, v, table, lens, good, max_q, out=out), want)
     ops.check_device_status()
+
+
+# ------------------------------------------------------------------------------------------------ outputs that lie over inputs
+@pytest.mark.parametrize("rows", [3, 60])
+def test_overlapping_memory_is_refused(rows):
+    """An output that lies over a part of the queries, keys or cache is refused, also when its shapes have been seen before; the queries' own place, and neighbours in one buffer, are
+    taken."""
+    hq, hkv, d, page = 8, 2, 64, 16
+    buf = torch.randn(((rows + 2) * (hq + 2 * hkv) * d,), device="cuda").to(F16)
+    w = (hq + 2 * hkv) * d
+    prod = buf[:rows * w].view(rows, w)
+    q, k, v = (x.unflatten(1, (-1, d)) for x in prod.split((hq * d, hkv * d, hkv * d), dim=1))
+    pool = torch.randn((16, 2, hkv, page, d), device="cuda").to(F16)
+    kc, vc = pool[:, 0], pool[:, 1]
+    table, lens, cu = _i32([[0, 1, 2, 3]]), _i32([rows]), _i32([0, rows])
+    attend = lambda **kw: ops.paged_attention(kw.get("q", q), kc, vc, table, lens, cu, rows, out=kw.get("out"))
+    dense = q.contiguous()
+    want = attend(q=dense)
+    shifted = torch.empty(dense.numel() + hq * d, dtype=F16, device="cuda")
+    a, b = shifted[:dense.numel()].view(dense.shape), shifted[hq * d:].view(dense.shape)
+    a.copy_(dense)
+    for _ in range(2):
+        for bad in (dict(q=a, out=b), dict(out=buf[8:8 + dense.numel()].view(dense.shape)), dict(q=dense, out=pool.flatten()[:dense.numel()].view(dense.shape))):
+            with pytest.raises(ValueError, match="overlap"):
+                attend(**bad)
+        assert torch.equal(attend(q=a, out=torch.empty_like(a)), want)
+    assert torch.equal(attend(q=a, out=a), want)
+    pos, slots = torch.arange(rows, device="cuda").to(torch.int32), torch.arange(rows, device="cuda").to(torch.int32)
+    inv, _ = ops.rope_frequencies(d)
+    put = lambda **kw: ops.rope_append(*(kw.get(n, t) for n, t in (("q", q), ("k", k), ("v", v))), pos, slots, inv, kw.get("kc", kc), kw.get("vc", vc), out=kw.get("out"))
+    turned = put()
+    wide = torch.as_strided(buf, (rows, hq, d), (w, d, 1), hkv * d)          # over the product's rows, two heads on
+    for bad in (dict(out=wide), dict(vc=kc), dict(k=pool.flatten()[:rows * hkv * d].view(rows, hkv, d))):
+        with pytest.raises(ValueError, match="overlap"):
+            put(**bad)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.rope(dense, pos, inv, out=torch.as_strided(dense, dense.shape, (d, rows * d, 1)))
+    assert put(out=q).data_ptr() == q.data_ptr() and torch.equal(q, turned)

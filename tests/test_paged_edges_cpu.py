@@ -1,0 +1,65 @@
+"""Host checks of the paged-cache operators at the edges of what their documentation allows (no GPU needed)."""
+import itertools
+import random
+
+import pytest
+import torch
+
+from kyojin_mac_b200 import ops
+
+
+# ------------------------------------------------------------------------------------------------ memory that a call reads and writes
+def _places(t):
+    """Element numbers of a view in its storage."""
+    n = torch.zeros(1, dtype=torch.long)
+    for s, st in zip(t.shape, t.stride()):
+        n = (n[:, None] + torch.arange(s) * st).flatten()
+    return set((n + t.storage_offset()).tolist())
+
+
+def _views(buf):
+    """Views of one buffer of 4096 values as callers make them: rows of a product, heads apart, transposed, shifted."""
+    for off, tokens, heads, d in itertools.product((0, 8, 16, 64, 200), (1, 3, 5), (1, 2, 4), (8, 16)):
+        for layout in ((heads * d, d), (96, d), (128, d), (128, 2 * d), (d, tokens * d), (64, 16), (200, d)):
+            t = torch.as_strided(buf, (tokens, heads, d), (*layout, 1), off)
+            if len(_places(t)) == t.numel():
+                yield t
+
+
+def test_overlap_is_found():
+    """A pair that shares an element is never taken for one that does not; the layouts that callers use are taken."""
+    buf, r = torch.zeros(4096, dtype=torch.float16), random.Random(1)
+    views = list(_views(buf))
+    found = taken = 0
+    for _ in range(20000):
+        a, b = r.choice(views), r.choice(views)
+        v = ops._Views([("q", a), ("out", b)], ["out"], ("q", "out"))
+        walk = lambda t: (t.storage_offset(), t.shape, [s for n, s in zip(t.shape, t.stride()) if n > 1])
+        same = walk(a) == walk(b)                                            # (the stride of a dimension of one is never used)
+        shared = bool(_places(a) & _places(b))
+        try:
+            v.check(a.data_ptr(), b.data_ptr())
+            assert not shared or same
+            taken += not shared
+        except ValueError:
+            found += shared
+    assert found > 1000 and taken > 1000
+
+
+def test_usual_layouts_pass():
+    t, hq, hkv, d, w = 5, 4, 2, 16, 128 + 8
+    buf = torch.zeros(4096, dtype=torch.float16)
+    q, k, v = (torch.as_strided(buf, (t, h, d), (w, d, 1), off) for h, off in ((hq, 0), (hkv, hq * d), (hkv, (hq + hkv) * d)))
+    pool = torch.zeros((3, 2, hkv, 16, d), dtype=torch.float16)              # pages outside, keys and values inside
+    kc, vc = pool[:, 0], pool[:, 1]
+    named = [("q", q), ("k", k), ("v", v), ("k_cache", kc), ("v_cache", vc), ("out", q)]
+    ptrs = [x.data_ptr() for _, x in named]
+    ops._Views(named, ["k_cache", "v_cache", "out"], ("q", "out")).check(*ptrs)
+    apart = torch.zeros((t, hq, 2, d), dtype=torch.float16)                  # heads of queries and output in turn
+    ops._Views([("q", apart[:, :, 0]), ("out", apart[:, :, 1])], ["out"], ("q", "out")).check(apart.data_ptr(), apart[:, :, 1].data_ptr())
+    for name, other in (("out", k), ("out", torch.as_strided(buf, (t, hq, d), (w, d, 1), 8)), ("out", torch.as_strided(buf, (t, hq, d), (hq * d, d, 1), 0)), ("v_cache", kc), ("k_cache", vc)):
+        bad = [(n, other if n == name else x) for n, x in named]
+        with pytest.raises(ValueError, match="overlap"):
+            ops._Views(bad, ["k_cache", "v_cache", "out"], ("q", "out")).check(*[x.data_ptr() for _, x in bad])
+    empty = torch.zeros((0, 4, 16), dtype=torch.float16)
+    ops._Views([("q", empty), ("out", empty)], ["out"], ("q", "out")).check(empty.data_ptr(), empty.data_ptr())
