@@ -30,7 +30,7 @@ extern "C" int kyb_paged_attention(const kyb_paged_attention_args* a, void* stre
     const int64_t pages = a->pages, ld_table = a->ld_table, cols = a->cols, batch = a->batch, tokens = a->tokens, max_q = a->max_q, window = a->window, sinks = a->sinks;
     for (int64_t n : {a->page, a->hq, a->hkv, a->d, a->dtype}) KYB_REQUIRE(n >= 0 && n <= 65535, "a size of %lld: out of range", (long long)n);
     const int page = (int)a->page, hq = (int)a->hq, hkv = (int)a->hkv, d = (int)a->d, dtype = (int)a->dtype;
-    const float scale = (float)a->scale;
+    const float scale2 = (float)a->scale * 1.4426950408889634f;          // what the kernels multiply with
     const size_t ws_bytes = a->ws_bytes < 0 ? 0 : (size_t)a->ws_bytes;
     KYB_REQUIRE(batch > 0 && batch < (1ll << 24) && tokens >= 0 && tokens < (1ll << 30) && max_q >= 0 && max_q <= (1 << 30), "batch=%lld tokens=%lld max_q=%lld: out of range", (long long)batch, (long long)tokens,
                 (long long)max_q);
@@ -42,7 +42,7 @@ extern "C" int kyb_paged_attention(const kyb_paged_attention_args* a, void* stre
                 (long long)pages);
     KYB_REQUIRE(cols > 0 && ld_table >= cols && cols <= (1 << 30) / page, "table of %lld columns (row stride %lld), %d tokens a page: out of range", (long long)cols, (long long)ld_table, page);
     KYB_REQUIRE(window >= 0 && sinks >= 0 && (window > 0 || sinks == 0), "window=%lld sinks=%lld: not negative, sinks only with a window", (long long)window, (long long)sinks);
-    KYB_REQUIRE(scale == scale && scale - scale == 0.f, "the scale is a finite number");
+    KYB_REQUIRE(scale2 - scale2 == 0.f, "scale=%g: a finite number, and so times log2(e) in 32 bits", a->scale);
     if (tokens == 0) return KYB_OK;
     KYB_REQUIRE(q && k_cache && v_cache && table && kv_lens && cu_q && out, "null pointer");
     for (int64_t s : {a->q_token, a->q_head, a->k_page, a->k_head, a->v_page, a->v_head, a->out_token, a->out_head})
@@ -55,7 +55,7 @@ extern "C" int kyb_paged_attention(const kyb_paged_attention_args* a, void* stre
     p.q = (const uint8_t*)q, p.o = (uint8_t*)out, p.q_t = a->q_token, p.q_h = a->q_head, p.o_t = a->out_token, p.o_h = a->out_head;
     p.table = (const int*)table, p.ld_table = ld_table, p.kv_lens = (const int*)kv_lens, p.cu_q = (const int*)cu_q;
     p.batch = (int)batch, p.tokens = (int)tokens, p.hq = hq, p.hkv = hkv, p.group = hq / hkv, p.pages = (int)pages, p.cap = (int)(cols * page);
-    p.window = (int)std::min<int64_t>(window, 1 << 30), p.sinks = (int)std::min<int64_t>(sinks, 1 << 30), p.scale2 = scale * 1.4426950408889634f, p.status = status;
+    p.window = (int)std::min<int64_t>(window, 1 << 30), p.sinks = (int)std::min<int64_t>(sinks, 1 << 30), p.scale2 = scale2, p.status = status;
     // a hidden score is -inf and stays so times the scale: 0 would make it NaN, the smallest normal number gives the same weights
     if (!(p.scale2 >= FLT_MIN || p.scale2 <= -FLT_MIN)) p.scale2 = FLT_MIN;
     p.page_log2 = 0, p.block_tokens = 0, p.parts = nullptr, p.notes = nullptr;

@@ -1,11 +1,12 @@
 """Host checks of the paged-cache operators at the edges of what their documentation allows (no GPU needed)."""
 import itertools
+import math
 import random
 
 import pytest
 import torch
 
-from kyojin_mac_b200 import ops
+from kyojin_mac_b200 import _lib, ops
 
 
 # ------------------------------------------------------------------------------------------------ memory that a call reads and writes
@@ -63,3 +64,24 @@ def test_usual_layouts_pass():
             ops._Views(bad, ["k_cache", "v_cache", "out"], ("q", "out")).check(*[x.data_ptr() for _, x in bad])
     empty = torch.zeros((0, 4, 16), dtype=torch.float16)
     ops._Views([("q", empty), ("out", empty)], ["out"], ("q", "out")).check(empty.data_ptr(), empty.data_ptr())
+
+
+# ------------------------------------------------------------------------------------------------ numbers
+@pytest.fixture(scope="module")
+def lib():
+    _lib.build()
+    return _lib.lib()
+
+
+P = 64                       # stands for an address that is 16-byte aligned; calls below are refused, or end for want of a device, before anything is read
+ATTENTION = dict(q=P, k=P, v=P, table=P, kv=P, cu=P, out=P, ws=P, q_t=128, q_h=64, k_p=1024, k_h=1024, v_p=1024, v_h=1024, o_t=128, o_h=64, pages=2, page=16, ld=3, cols=3, batch=1, tokens=0,
+                 max_q=3, hq=2, hkv=1, d=64, dt=1, window=0, sinks=0, wsn=1 << 30, scale=0.1)
+
+
+def test_scale_in_powers_of_two(lib):
+    """The kernels use scale * log2(e): a scale that is finite itself but not so (above 2.36e38) is refused; the largest that is passes (no tokens: nothing to do)."""
+    call = lambda scale: lib.kyb_paged_attention(_lib.PAGED_ATTENTION_ARGS.pack(*{**ATTENTION, "scale": scale}.values()), None)
+    for bad in (2.4e38, -2.4e38, 3.4e38, math.inf, -math.inf, math.nan):
+        assert call(bad) == _lib.EINVAL, bad
+    for good in (2.3e38, -2.3e38, 0.0, 1e-45, 1.0):
+        assert call(good) == _lib.OK, good
