@@ -2,6 +2,7 @@
 #include <stdarg.h>
 #include <string.h>
 
+#include <atomic>
 #include <mutex>
 #include <unordered_map>
 
@@ -31,6 +32,14 @@ unsigned int* kyb_device_status_word() {
         g_status_words[dev] = (unsigned int*)p;
     }
     return g_status_words[dev];
+}
+
+int kyb_sm_count() {
+    static std::atomic<int> known[64];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    if ((n = known[dev].load(std::memory_order_relaxed)) == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) known[dev].store(n, std::memory_order_relaxed);
+    return n;
 }
 
 int kyb_allow_smem(const void* kern) {

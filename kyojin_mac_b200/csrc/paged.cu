@@ -345,7 +345,7 @@ extern "C" int kyb_rope_append(const kyb_rope_append_args* a, void* stream) {
     p.hq = hq, p.hkv = hkv, p.d = d, p.rot = rot, p.mscale = mscale;
     const int units = (hq + hkv) * (rot / 16 + ((d - rot) / 8 + 1) / 2) + hkv * ((d / 8 + 1) / 2);
     int parts = 1;                                                        // parts of a token's heads: until every SM has two CTAs or a thread has one unit
-    while (tokens * parts < 296 && parts * kyb::RP_THREADS < units) parts *= 2;
+    while (tokens * parts < 2 * kyb_sm_count() && parts * kyb::RP_THREADS < units) parts *= 2;
     p.parts = parts;
     // as many threads as a CTA's units fill in equal turns (8191 tokens of 8 / 1 heads of 128, 80 units: 18 us by 256 threads, 12.3 by 96)
     const int share = (units + parts - 1) / parts, turns = (share + kyb::RP_THREADS - 1) / kyb::RP_THREADS;

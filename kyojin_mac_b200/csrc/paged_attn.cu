@@ -3,24 +3,14 @@
 #include <float.h>
 
 #include <algorithm>
-#include <atomic>
 
 #include "paged_attn.cuh"
-
-// SMs of the current device (0: none), asked once per device
-static int sm_count() {
-    static std::atomic<int> known[64];
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-    if ((n = known[dev].load(std::memory_order_relaxed)) == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) known[dev].store(n, std::memory_order_relaxed);
-    return n;
-}
 
 extern "C" size_t kyb_paged_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t max_q, int64_t cols, int page, int hq, int hkv, int d) {
     (void)batch, (void)cols, (void)page;
     if (tokens <= 0 || hkv <= 0 || hq < hkv || hq / hkv > 128) return 0;
     const int64_t rows = std::max<int64_t>(max_q, 1) * (hq / hkv);
-    return rows <= KYB_DECODE_ROWS ? kyb_attn_decode_scratch(d, (int)rows, sm_count()) : kyb_attn_prefill_scratch(d, hq / hkv, sm_count());
+    return rows <= KYB_DECODE_ROWS ? kyb_attn_decode_scratch(d, (int)rows, kyb_sm_count()) : kyb_attn_prefill_scratch(d, hq / hkv, kyb_sm_count());
 }
 
 extern "C" int kyb_paged_attention(const kyb_paged_attention_args* a, void* stream) {
@@ -60,7 +50,7 @@ extern "C" int kyb_paged_attention(const kyb_paged_attention_args* a, void* stre
     if (!(p.scale2 >= FLT_MIN || p.scale2 <= -FLT_MIN)) p.scale2 = FLT_MIN;
     p.page_log2 = 0, p.block_tokens = 0, p.parts = nullptr, p.notes = nullptr;
     while ((1 << p.page_log2) < page) ++p.page_log2;
-    c.k = k_cache, c.v = v_cache, c.k_p = a->k_page, c.k_h = a->k_head, c.v_p = a->v_page, c.v_h = a->v_head, c.tokens = tokens, c.d = d, c.dtype = dtype, c.page = page, c.sms = sm_count();
+    c.k = k_cache, c.v = v_cache, c.k_p = a->k_page, c.k_h = a->k_head, c.v_p = a->v_page, c.v_h = a->v_head, c.tokens = tokens, c.d = d, c.dtype = dtype, c.page = page, c.sms = kyb_sm_count();
     c.st = (cudaStream_t)stream;
     KYB_REQUIRE(c.sms > 0, "no CUDA device");
     const size_t need = kyb_paged_attention_workspace_bytes(batch, tokens, max_q, cols, page, hq, hkv, d);
