@@ -7,6 +7,7 @@ from typing import NamedTuple
 
 import numpy as np
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _lib, flags as F
 from .layout import FMT_ID, padded_rows
@@ -522,12 +523,17 @@ def _table(t, page):
         raise ValueError(f"{page} tokens a page: 16, 32, 64, 128 or 256")
 
 
+def _no_gradient(t, name):
+    """There is no backward here: a tensor that takes part in differentiation is refused rather than cut off from it."""
+    if (t.requires_grad and torch.is_grad_enabled()) or (_forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None):
+        raise ValueError(f"{name} requires a gradient: the paged cache serves inference (use torch.no_grad or detach)")
+
+
 def _heads(t, name):
     """[tokens, heads, d] of a 16-bit type, heads dense, strides that 16-byte accesses can follow."""
     if t.dtype not in (torch.float16, torch.bfloat16) or t.dim() != 3:
         raise ValueError(f"{name} must be float16 or bfloat16 [tokens, heads, d], got {t.dtype} {tuple(t.shape)}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} requires a gradient: the paged cache serves inference (use torch.no_grad or detach)")
+    _no_gradient(t, name)
     if t.numel() and (t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16):
         raise ValueError(f"{name}: heads must be dense, strides multiples of 8 elements, the start 16-byte aligned; got strides {t.stride()}")
 
@@ -542,6 +548,7 @@ def _own_rows(t, name):
 def _cache(t, name, like=None):
     if t.dtype not in (torch.float16, torch.bfloat16) or t.dim() != 4 or t.shape[2] not in (16, 32, 64, 128, 256) or (like is not None and (t.shape != like.shape or t.dtype != like.dtype)):
         raise ValueError(f"{name} must be float16 or bfloat16 [pages, kv heads, 16 .. 256 (a power of two), d], keys and values alike, got {t.dtype} {tuple(t.shape)}")
+    _no_gradient(t, name)
     p, h, n, d = t.shape
     if t.numel() == 0 or t.stride(3) != 1 or t.stride(2) != d or t.data_ptr() % 16 or (p > 1 and (t.stride(0) % 8 or t.stride(0) < n * d)) or (h > 1 and (t.stride(1) % 8 or t.stride(1) < n * d)):
         raise ValueError(f"{name}: the tokens of a page and head must be dense, strides multiples of 8 elements, the start 16-byte aligned; got strides {t.stride()}")
@@ -709,6 +716,7 @@ def _rope_check(key, q, k, v, positions, slots, inv_freq, kc, vc, interleaved, m
     _heads(q, "q"), _i32(positions, "positions", q.shape[0])
     if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq is contiguous float32 [rot / 2]")
+    _no_gradient(inv_freq, "inv_freq")
     T, hq, d = q.shape
     if out is not None:
         _heads(out, "out"), _own_rows(out, "out")
@@ -730,12 +738,12 @@ def _rope_check(key, q, k, v, positions, slots, inv_freq, kc, vc, interleaved, m
 
 def _rope_call(q, k, v, positions, slots, inv_freq, kc, vc, interleaved, mscale, out):
     """The queries turned (into `out`), keys and values into the cache where there are any."""
-    dev, grad = q.get_device(), q.requires_grad
+    dev, grad = q.get_device(), q.requires_grad or inv_freq.requires_grad or (out is not None and out.requires_grad) or _forward_ad._current_level >= 0
     if k is None:
         key = (dev, q.shape, q.stride(), q.dtype, positions.shape, positions.dtype, positions.is_contiguous(), inv_freq.shape, inv_freq.dtype, positions.get_device(), inv_freq.get_device(), interleaved,
                mscale)
     else:
-        grad = grad or k.requires_grad or v.requires_grad
+        grad = grad or k.requires_grad or v.requires_grad or kc.requires_grad or vc.requires_grad
         key = (dev, q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, positions.shape, positions.dtype, positions.is_contiguous(), slots.shape, slots.dtype,
                slots.is_contiguous(), inv_freq.shape, inv_freq.dtype, kc.shape, kc.is_contiguous() or kc.stride(), kc.dtype, vc.shape, vc.is_contiguous() or vc.stride(), vc.dtype, k.get_device(),
                v.get_device(), positions.get_device(), slots.get_device(), inv_freq.get_device(), kc.get_device(), vc.get_device(), interleaved, mscale)
@@ -820,7 +828,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
            v_cache.is_contiguous() or v_cache.stride(), v_cache.dtype, table.shape, table.is_contiguous() or table.stride(), table.dtype, kv_lens.shape, kv_lens.dtype, kv_lens.is_contiguous(),
            cu_q.shape, cu_q.dtype, cu_q.is_contiguous(), max_q, scale, window, sinks, k_cache.get_device(), v_cache.get_device(), table.get_device(), kv_lens.get_device(), cu_q.get_device(),
            None if out is None else (out.shape, out.stride(), out.dtype, out.get_device()))
-    known = None if q.requires_grad else _passed.get(key)
+    grad = q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or (out is not None and out.requires_grad) or _forward_ad._current_level >= 0
+    known = None if grad else _passed.get(key)
     if known is None:
         known = _attention_check(key, q, k_cache, v_cache, table, kv_lens, cu_q, max_q, scale, window, sinks, out)
     if dev != torch.cuda.current_device() if _cur_device is None else dev != _cur_device():

@@ -135,3 +135,31 @@ def test_overlapping_memory_is_refused(rows):
     with pytest.raises(ValueError, match="overlap"):
         ops.rope(dense, pos, inv, out=torch.as_strided(dense, dense.shape, (d, rows * d, 1)))
     assert put(out=q).data_ptr() == q.data_ptr() and torch.equal(q, turned)
+
+
+# ------------------------------------------------------------------------------------------------ no backward
+def test_whatever_takes_part_in_differentiation_is_refused():
+    """Queries, keys, values, caches, outputs and frequencies that require a gradient or carry a forward-mode tangent: also when the same shapes have passed before; without
+    gradients they are taken."""
+    import torch.autograd.forward_ad as fwd
+    x = lambda *s: torch.randn(s, device="cuda").to(F16)
+    inv, _ = ops.rope_frequencies(64)
+    pos = _i32([0, 1, 2])
+    rope = dict(q=x(3, 4, 64), k=x(3, 2, 64), v=x(3, 2, 64), inv_freq=inv, k_cache=x(2, 2, 16, 64), v_cache=x(2, 2, 16, 64), out=x(3, 4, 64))
+    attend = dict(q=x(3, 4, 64), k_cache=x(2, 2, 16, 64), v_cache=x(2, 2, 16, 64), out=x(3, 4, 64))
+    alone = dict(x=x(3, 4, 64), inv_freq=inv, out=x(3, 4, 64))
+    calls = ((lambda **kw: ops.rope_append(positions=pos, slots=pos, **kw), rope), (lambda **kw: ops.rope(positions=pos, **kw), alone),
+             (lambda **kw: ops.paged_attention(table=_i32([[0]]), kv_lens=_i32([3]), cu_q=_i32([0, 3]), max_q=3, **kw), attend))
+    for call, good in calls:
+        for turn in range(2):
+            for name, t in good.items():
+                leaf = t.clone().requires_grad_()
+                with pytest.raises(ValueError, match="gradient"):
+                    call(**{**good, name: leaf})
+                with torch.no_grad():
+                    call(**{**good, name: leaf})
+                with fwd.dual_level():
+                    call(**good)
+                    with pytest.raises(ValueError, match="gradient"):
+                        call(**{**good, name: fwd.make_dual(t, torch.ones_like(t))})
+            call(**good)
