@@ -196,7 +196,7 @@ static inline int kyb_make_cache_map(CUtensorMap* tm, const void* base, int dtyp
     const cuuint32_t box[5] = {64, (cuuint32_t)box_tokens, (cuuint32_t)box_halves, 1, 1};
     const CUresult r = kyb_encode_map(tm, dtype == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (r != CUDA_SUCCESS) {
-        kyb_set_error("cuTensorMapEncodeTiled failed with CUresult %d (cache %p: %lld pages, %d heads, %d tokens of %d values, strides %lld, %lld)", (int)r, base, (long long)pages, heads, page,
+        kyb_set_error("%s CUresult %d (cache %p: %lld pages, %d heads, %d tokens of %d values, strides %lld, %lld)", kyb_encode_problem(r), (int)r, base, (long long)pages, heads, page,
                       d, (long long)page_stride, (long long)head_stride);
         return KYB_ECUDA;
     }

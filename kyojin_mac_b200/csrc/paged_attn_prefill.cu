@@ -631,7 +631,7 @@ int make_query_map(CUtensorMap* tm, const KybAttnCall& c, int qtoks) {
     const cuuint32_t box[5] = {64, 1, (cuuint32_t)p.group, 1, (cuuint32_t)qtoks};
     const CUresult r = kyb_encode_map(tm, c.dtype == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, p.q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (r != CUDA_SUCCESS) {
-        kyb_set_error("cuTensorMapEncodeTiled failed with CUresult %d (queries %p: %lld tokens, %d x %d heads of %d, strides %lld, %lld)", (int)r, (const void*)p.q, (long long)c.tokens, p.hkv,
+        kyb_set_error("%s CUresult %d (queries %p: %lld tokens, %d x %d heads of %d, strides %lld, %lld)", kyb_encode_problem(r), (int)r, (const void*)p.q, (long long)c.tokens, p.hkv,
                       p.group, c.d, (long long)token, (long long)head);
         return KYB_ECUDA;
     }

@@ -37,6 +37,11 @@ static inline CUresult kyb_encode_map(CUtensorMap* tm, CUtensorMapDataType dt, c
     return r;
 }
 
+// what went wrong, for the error text (the encoder itself never answers CUDA_ERROR_NOT_FOUND: that is a driver without it)
+static inline const char* kyb_encode_problem(CUresult r) {
+    return r == CUDA_ERROR_NOT_FOUND ? "cuTensorMapEncodeTiled is not available from this driver:" : "cuTensorMapEncodeTiled failed with";
+}
+
 // 2-D row-major tensor [rows, cols] of `elem_bytes`-wide elements, row stride `ld_bytes`; box [box_rows, box_cols]; 128-byte swizzle by default
 // (box_cols * elem_bytes must equal the swizzle width). Out-of-range parts of a box are filled with zeros on loads and dropped on stores.
 static inline int kyb_make_tmap_2d(CUtensorMap* tm, CUtensorMapDataType dt, int elem_bytes, const void* base, uint64_t rows, uint64_t cols, uint64_t ld_bytes,
@@ -47,7 +52,7 @@ static inline int kyb_make_tmap_2d(CUtensorMap* tm, CUtensorMapDataType dt, int 
     (void)elem_bytes;
     const CUresult r = kyb_encode_map(tm, dt, 2, base, dims, strides, box, swizzle);
     if (r != CUDA_SUCCESS) {
-        kyb_set_error("cuTensorMapEncodeTiled failed with CUresult %d (base %p rows %llu cols %llu ld %llu box %u x %u)", (int)r, base, (unsigned long long)rows,
+        kyb_set_error("%s CUresult %d (base %p rows %llu cols %llu ld %llu box %u x %u)", kyb_encode_problem(r), (int)r, base, (unsigned long long)rows,
                       (unsigned long long)cols, (unsigned long long)ld_bytes, box_rows, box_cols);
         return KYB_ECUDA;
     }

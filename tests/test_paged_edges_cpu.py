@@ -1,7 +1,9 @@
 """Host checks of the paged-cache operators at the edges of what their documentation allows (no GPU needed)."""
 import itertools
 import math
+import os
 import random
+import subprocess
 
 import pytest
 import torch
@@ -85,3 +87,31 @@ def test_scale_in_powers_of_two(lib):
         assert call(bad) == _lib.EINVAL, bad
     for good in (2.3e38, -2.3e38, 0.0, 1e-45, 1.0):
         assert call(good) == _lib.OK, good
+
+
+# ------------------------------------------------------------------------------------------------ error texts
+def test_a_driver_without_the_encoder_is_named(tmp_path):
+    """Where the driver has no tensor-map encoder (as here, where there is no driver), the error says so instead of a bare number."""
+    src = tmp_path / "maps.cpp"
+    src.write_text("""
+#include <stdarg.h>
+#include <stdio.h>
+#include "tc_common.cuh"
+void kyb_set_error(const char* fmt, ...) { va_list a; va_start(a, fmt); vprintf(fmt, a); va_end(a); printf("\\n"); }
+int main() {
+    if (kyb_get_encode_tiled()) return 77;
+    CUtensorMap m;
+    return kyb_make_tmap_2d(&m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, (void*)256, 128, 64, 128, 64, 64) == KYB_ECUDA ? 0 : 1;
+}
+""")
+    csrc = os.path.join(os.path.dirname(os.path.abspath(_lib.__file__)), "csrc")
+    cuda = "/usr/local/cuda"
+    if not os.path.exists(cuda + "/include/cuda.h"):
+        pytest.skip("no CUDA headers")
+    exe = str(tmp_path / "maps")
+    subprocess.run(["g++", "-std=c++17", "-I", csrc, "-I", os.path.join(csrc, "..", "..", "include"), "-I", cuda + "/include", str(src), "-o", exe, "-L", cuda + "/lib64", "-lcudart_static", "-ldl", "-lrt",
+                    "-lpthread"], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True)
+    if r.returncode == 77:
+        pytest.skip("this driver has the encoder")
+    assert r.returncode == 0 and "not available from this driver" in r.stdout, r
