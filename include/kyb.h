@@ -266,8 +266,8 @@ typedef struct {
     int64_t free_cap, ld_table, batch, cols, page, rows;
 } kyb_paged_step_args;
 int kyb_paged_step(const kyb_paged_step_args* args, void* stream);
-/* pages of the requests with which[r] != 0 (uint8 [batch]) go back to the free list; their table entries become -1, their lengths 0. A request whose pages would
- * overflow the list keeps them and is counted in refused [1]. */
+/* pages of the requests with which[r] != 0 (uint8 [batch]) go back to the free list; their table entries become -1, their lengths 0. A request whose pages, behind
+ * those of the others before it, would overflow the list keeps them and is counted in refused [1]; one that holds no page is not held up. */
 int kyb_paged_release(void* lens, const void* which, void* table, int64_t ld_table, int64_t batch, int64_t cols, int page, void* free_pages, int64_t free_cap,
                       void* free_count, void* refused, void* stream);
 /* rotary positions and cache append: the pairs of the first rot values of every query and key head (interleaved: (2 i, 2 i + 1), else (i, i + rot / 2)) turned by

@@ -148,24 +148,24 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_step_kernel(const StepPar
     }
 }
 
-// Pages of the requests with which[r] != 0 go back to the free list, in request order; their table entries read -1 and their lengths 0 afterwards. A request whose
-// pages would overflow the list (a page freed twice) keeps them and is counted in *refused. One CTA.
+// Pages of the requests with which[r] != 0 go back to the free list, in request order; their table entries read -1 and their lengths 0 afterwards. A request whose pages, behind
+// those of all of them before it, would overflow the list (a page freed twice) keeps them and is counted in *refused; one that holds no page is not held up. One CTA.
 __global__ void __launch_bounds__(PS_THREADS, 1) paged_release_kernel(int* lens, const uint8_t* which, int* table, int64_t ld_table, int64_t batch, int64_t cols, int page,
                                                                       int* free_pages, int* free_count, int64_t free_cap, int* refused) {
     __shared__ StepShared s;
-    __shared__ long long total;
+    __shared__ long long total, asked;                                  // pages that go back, and that would, of the chunk
     const int tid = threadIdx.x;
-    long long count = max(0ll, min((long long)*free_count, (long long)free_cap)), missed = 0;
+    long long count = max(0ll, min((long long)*free_count, (long long)free_cap)), room = free_cap - count, missed = 0;
     for (int64_t c0 = 0; c0 < batch; c0 += PS_THREADS) {
         const int n = (int)min((int64_t)PS_THREADS, batch - c0);
         const bool on = tid < n && which[c0 + tid];
         const long long len = on ? max(0, lens[c0 + tid]) : 0, pages = min((len + page - 1) / page, (long long)cols);
         const long long end = block_scan(on ? pages : 0, s.warp_sum[0]);
-        const bool fits = on && count + end <= free_cap;                // sums grow, so the requests that fit are the first ones
+        const bool fits = on && (pages == 0 || end <= room);            // sums grow, so the requests that fit are the first ones, over all chunks
         const long long kept = block_scan(fits ? pages : 0, s.warp_sum[1]);
         const int miss = __syncthreads_count(on && !fits);
         if (tid < n) s.need_end[tid] = (int)kept;
-        if (tid == PS_THREADS - 1) total = kept;
+        if (tid == PS_THREADS - 1) total = kept, asked = end;
         __syncthreads();
         for (int j = tid; j < (int)total; j += PS_THREADS) {
             const int r = first_above(s.need_end, n, j), k = j - (r ? s.need_end[r - 1] : 0);
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_release_kernel(int* lens,
             *e = -1;
         }
         if (fits) lens[c0 + tid] = 0;
-        count += total, missed += miss;
+        count += total, room -= asked, missed += miss;
         __syncthreads();
     }
     if (tid == 0) *free_count = (int)count, *refused = (int)missed;

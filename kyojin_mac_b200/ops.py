@@ -659,7 +659,7 @@ def paged_step(table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor, 
 
 def paged_release(table: torch.Tensor, lens: torch.Tensor, which: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor, page: int) -> torch.Tensor:
     """The pages of the requests with which[r] (bool [batch]) go back to the free list, in place: their lengths become 0, their table entries -1. Returns int32 [1]:
-    requests whose pages would overflow the list (they keep them)."""
+    requests whose pages, behind those of the others before them, would overflow the list (they keep them; one without pages is not held up)."""
     guard = _place(table, lens, which, free_pages, free_count)
     _table(table, page)
     b, cols = table.shape

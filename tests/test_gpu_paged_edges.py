@@ -163,3 +163,33 @@ def test_whatever_takes_part_in_differentiation_is_refused():
                     with pytest.raises(ValueError, match="gradient"):
                         call(**{**good, name: fwd.make_dual(t, torch.ones_like(t))})
             call(**good)
+
+
+# ------------------------------------------------------------------------------------------------ pages given back
+@pytest.mark.parametrize("b,room", [(2500, 10 ** 6), (2500, 900), (2500, 0), (1024, 500), (1025, 40), (30, 11)])
+def test_release_into_a_short_list(b, room):
+    """A list without room for all: the requests up to the one that overflows it give their pages back, those behind it keep theirs (wherever a thousand requests end), and a request
+    that holds no page is served."""
+    r = random.Random(b + room)
+    page, cols = 16, 5
+    lens = [r.choice((0, r.randint(1, 70))) for _ in range(b)]
+    need = [-(-n // page) for n in lens]
+    ids = r.sample(range(10 ** 6), sum(need) + 3)
+    at = [sum(need[:i]) for i in range(b)]
+    table = [ids[a:a + n] + [-1] * (cols - n) for a, n in zip(at, need)]
+    which = [r.random() < 0.7 for _ in range(b)]
+    cap = 3 + min(room, sum(n for n, w in zip(need, which) if w))
+    free, asked, refused, lens_after, table_after = ids[-3:], 0, 0, list(lens), [list(t) for t in table]
+    for i in range(b):
+        if not which[i]:
+            continue
+        asked += need[i]
+        if need[i] and 3 + asked > cap:
+            refused += 1
+            continue
+        free += table[i][:need[i]]
+        lens_after[i], table_after[i] = 0, [-1] * cols
+    t, ln, ct, fr = _i32(table), _i32(lens), _i32([3]), _i32(ids[-3:] + [-9] * (cap - 3))
+    got = ops.paged_release(t, ln, torch.tensor(which, device="cuda"), fr, ct, page).item()
+    assert got == refused and ct.item() == len(free) and fr.tolist() == free + [-9] * (cap - len(free))
+    assert ln.tolist() == lens_after and t.tolist() == table_after
