@@ -534,8 +534,13 @@ def _heads(t, name):
     if t.dtype not in (torch.float16, torch.bfloat16) or t.dim() != 3:
         raise ValueError(f"{name} must be float16 or bfloat16 [tokens, heads, d], got {t.dtype} {tuple(t.shape)}")
     _no_gradient(t, name)
-    if t.numel() and (t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16):
+    if t.numel() and (t.stride(2) != 1 or any(s % 8 for s in _steps(t)) or t.data_ptr() % 16):
         raise ValueError(f"{name}: heads must be dense, strides multiples of 8 elements, the start 16-byte aligned; got strides {t.stride()}")
+
+
+def _steps(t):
+    """The two outer strides; that of a dimension of one, which may be anything, as 0."""
+    return tuple(s if n > 1 else 0 for n, s in zip(t.shape[:2], t.stride()))
 
 
 def _own_rows(t, name):
@@ -728,11 +733,11 @@ def _rope_check(key, q, k, v, positions, slots, inv_freq, kc, vc, interleaved, m
         _heads(k, "k"), _heads(v, "v"), _cache(kc, "k_cache"), _cache(vc, "v_cache", kc), _i32(slots, "slots", T)
         if k.shape != (T, kc.shape[1], d) or v.shape != k.shape or kc.shape[3] != d or not q.dtype == k.dtype == v.dtype == kc.dtype:
             raise ValueError(f"q [T, heads, d], k and v [T, kv heads, d] and the cache go together, in one type: got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}, {tuple(kc.shape)}")
-        ks, vs, kcs, vcs = k.stride()[:2], v.stride()[:2], kc.stride()[:2], vc.stride()[:2]
+        ks, vs, kcs, vcs = _steps(k), _steps(v), _steps(kc), _steps(vc)
         pages, hkv, page = kc.shape[:3]
-    os_ = (hq * d, d) if out is None else out.stride()[:2]
+    os_ = (hq * d, d) if out is None else _steps(out)
     views = [(n, t) for n, t in (("q", q), ("k", k), ("v", v), ("k_cache", kc), ("v_cache", vc), ("out", out)) if t is not None]
-    return _remember(key, (_lib.ROPE_APPEND_SPLIT[1].pack(*q.stride()[:2], *ks, *vs, *os_, *kcs, *vcs, T, hq, hkv, d, 2 * inv_freq.shape[0], 1 if interleaved else 0, _DT[q.dtype], pages, page,
+    return _remember(key, (_lib.ROPE_APPEND_SPLIT[1].pack(*_steps(q), *ks, *vs, *os_, *kcs, *vcs, T, hq, hkv, d, 2 * inv_freq.shape[0], 1 if interleaved else 0, _DT[q.dtype], pages, page,
                                                           mscale), _Views(views, [n for n, _ in views if n in ("k_cache", "v_cache", "out")], ("q", "out"))))
 
 
@@ -809,9 +814,9 @@ def _attention_check(key, q, kc, vc, table, kv_lens, cu_q, max_q, scale, window,
             raise ValueError("out has the queries' shape and type")
     with torch.cuda.device(q.device):
         need = _lib.lib().kyb_paged_attention_workspace_bytes(b, T, max_q, cols, page, hq, hkv, d)
-    os_ = (hq * d, d) if out is None else out.stride()[:2]
+    os_ = (hq * d, d) if out is None else _steps(out)
     views = None if out is None else _Views([("q", q), ("k_cache", kc), ("v_cache", vc), ("out", out)], ["out"], ("q", "out"))
-    return _remember(key, (need, views, _lib.PAGED_ATTENTION_SPLIT[1].pack(*q.stride()[:2], *kc.stride()[:2], *vc.stride()[:2], *os_, pages, page, max(table.stride(0), cols), cols, b, T, max_q, hq, hkv,
+    return _remember(key, (need, views, _lib.PAGED_ATTENTION_SPLIT[1].pack(*_steps(q), *_steps(kc), *_steps(vc), *os_, pages, page, max(table.stride(0), cols), cols, b, T, max_q, hq, hkv,
                                                                     d, _DT[q.dtype], window, sinks, need, d ** -0.5 if scale is None else scale)))
 
 

@@ -193,3 +193,32 @@ def test_release_into_a_short_list(b, room):
     got = ops.paged_release(t, ln, torch.tensor(which, device="cuda"), fr, ct, page).item()
     assert got == refused and ct.item() == len(free) and fr.tolist() == free + [-9] * (cap - len(free))
     assert ln.tolist() == lens_after and t.tolist() == table_after
+
+
+# ------------------------------------------------------------------------------------------------ dimensions of one
+@pytest.mark.parametrize("hq", [1, 4, 40])
+def test_strides_of_dimensions_of_one(hq):
+    """One token of rows of an odd width, one head, one page: a stride that nothing steps by may be anything, in inputs, caches and outputs."""
+    d, page = 64, 16
+    x = lambda *s: torch.randn(s, device="cuda").to(F16)
+
+    def odd(t):
+        """The same values with strides of 1001 at dimensions of one."""
+        return torch.as_strided(t, t.shape, [s if n > 1 else 1001 for n, s in zip(t.shape, t.stride())])
+    inv, _ = ops.rope_frequencies(d)
+    pos, one = _i32([5]), _i32([[0]])
+    q, k, v, kc, vc = x(1, hq, d), x(1, 1, d), x(1, 1, d), x(1, 1, page, d), x(1, 1, page, d)
+    attend = lambda f: ops.paged_attention(f(q), f(kc), f(vc), one, _i32([6]), _i32([0, 1]), 1, out=f(torch.zeros_like(q)))
+    turn = lambda f: ops.rope(f(q), pos, inv, out=f(torch.zeros_like(q)))
+
+    def put(f):
+        c, w = kc.clone(), vc.clone()
+        return ops.rope_append(f(q), f(k), f(v), pos, pos, inv, f(c), f(w), out=f(torch.zeros_like(q))), c, w
+    for call in (attend, turn, put):
+        for order in ((odd, lambda t: t), (lambda t: t, odd)):
+            ops._passed.clear()                                              # whichever is seen first
+            a, b = (call(f) for f in order)
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+    many = x(30, 1, d)                                                       # several tokens of one head, and one request of one page
+    a, b = (ops.paged_attention(f(many), f(x2), f(x3), _i32([[0, 0]]), _i32([30]), _i32([0, 30]), 30) for f, x2, x3 in ((odd, kc, vc), (lambda t: t, kc, vc)))
+    assert torch.equal(a, b)
