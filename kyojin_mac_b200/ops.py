@@ -687,11 +687,16 @@ def rope_frequencies(rot: int, base: float = 10000.0, scaling: dict | None = Non
     {"type": "yarn", "factor", "original_context", "beta_fast" (32), "beta_slow" (1)}: the same with a ramp over the pair's index, and mscale = 0.1 ln(factor) + 1."""
     if rot < 16 or rot % 16:
         raise ValueError(f"rot={rot}: a multiple of 16")
-    if not base > 1.0:
-        raise ValueError("the base is above 1")
+    if not base > 1.0 or not math.isfinite(base):
+        raise ValueError("the base is a finite number above 1")
     i = torch.arange(0, rot, 2, dtype=torch.float64)
     inv, mscale = base ** (-i / rot), 1.0
     if scaling is not None:
+        def number(name, default=None, zero=False):
+            v = scaling.get(name, default)
+            if v is None or not 0.0 <= float(v) < math.inf or (float(v) == 0.0 and not zero):
+                raise ValueError(f"a scaling of type {kind!r} has a positive {name}, got {v}")
+            return float(v)
         kind, f = scaling.get("type"), float(scaling.get("factor", 0.0))
         if not f >= 1.0 or not math.isfinite(f):
             raise ValueError("a scaling has a factor of 1 at least")
@@ -700,13 +705,15 @@ def rope_frequencies(rot: int, base: float = 10000.0, scaling: dict | None = Non
         elif kind == "ntk":
             inv = (base * f ** (rot / (rot - 2))) ** (-i / rot)
         elif kind == "llama3":
-            low, high, ctx = (float(scaling[k]) for k in ("low_freq_factor", "high_freq_factor", "original_context"))
+            low, high, ctx = number("low_freq_factor", zero=True), number("high_freq_factor"), number("original_context")
             if not high > low:
                 raise ValueError("high_freq_factor is above low_freq_factor")
             keep = ((ctx * inv / (2 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
             inv = inv * keep + inv / f * (1 - keep)
         elif kind == "yarn":
-            ctx, fast, slow = float(scaling["original_context"]), float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+            ctx, fast, slow = number("original_context"), number("beta_fast", 32.0), number("beta_slow", 1.0)
+            if not fast > slow:
+                raise ValueError("a scaling's beta_fast is above its beta_slow")
             index = lambda turns: rot * math.log(ctx / (turns * 2 * math.pi)) / (2 * math.log(base))          # pair that makes so many turns in the context
             a, b = max(math.floor(index(fast)), 0), min(math.ceil(index(slow)), rot - 1)
             keep = 1.0 - ((torch.arange(rot // 2, dtype=torch.float64) - a) / max(b - a, 0.001)).clamp(0.0, 1.0)

@@ -115,3 +115,20 @@ int main() {
     if r.returncode == 77:
         pytest.skip("this driver has the encoder")
     assert r.returncode == 0 and "not available from this driver" in r.stdout, r
+
+
+@pytest.mark.parametrize("scaling", [
+    {"type": "llama3", "factor": 8.0}, {"type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0}, {"type": "yarn", "factor": 4.0},
+    {"type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0, "original_context": 0}, {"type": "yarn", "factor": 4.0, "original_context": 0},
+    {"type": "yarn", "factor": 4.0, "original_context": -5}, {"type": "yarn", "factor": 4.0, "original_context": math.inf}, {"type": "yarn", "factor": 4.0, "original_context": 4096, "beta_slow": 0},
+    {"type": "yarn", "factor": 4.0, "original_context": 4096, "beta_fast": 1, "beta_slow": 32}, {"type": "linear"}, {}])
+def test_scalings_that_lack_a_number(scaling):
+    """A scaling without one of its numbers, or with one that means nothing, is refused as any other argument is."""
+    with pytest.raises(ValueError, match="scaling|factor"):
+        ops.rope_frequencies(64, 10000.0, scaling, "cpu")
+
+
+def test_base_is_finite():
+    for bad in (math.inf, math.nan, 1.0, -5.0):
+        with pytest.raises(ValueError, match="base"):
+            ops.rope_frequencies(64, bad, device="cpu")
