@@ -138,7 +138,8 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_step_kernel(const StepPar
     }
     // rows behind the last request
     for (int64_t t = min(rows0, (long long)p.rows) + (int64_t)cta * PS_THREADS + tid; t < p.rows; t += (int64_t)ctas * PS_THREADS) p.positions[t] = -1, p.slots[t] = -1;
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");        // every CTA has read the state
+    // every CTA has read the state (not the .aligned form: the threads of a warp come out of the loop above at their own times)
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
     if (cta) return;
     if (tid == 0) *p.count_out = (int)(count - taken), *p.refused = (int)refused;
     // a request that was not served keeps its length; one that was has it in kv_lens (0 there: it holds and brings nothing)
