@@ -70,6 +70,16 @@ __host__ __device__ constexpr bool kyb_has_mins16(int fmt) { return fmt == KYB_F
 // ------------------------------------------------------------------------------------------------ device side
 namespace kyb {
 
+// smallest i with v[i] > x (v not decreasing, v[n - 1] > x)
+__device__ __forceinline__ int first_above(const int* v, int n, int x) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (v[mid] > x) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+}
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {

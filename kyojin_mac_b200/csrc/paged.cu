@@ -71,16 +71,6 @@ __device__ __forceinline__ long long block_scan(long long a, long long* sums) {
     return warp ? a + sums[warp - 1] : a;
 }
 
-// smallest i with v[i] > x (v not decreasing, v[n - 1] > x)
-__device__ __forceinline__ int first_above(const int* v, int n, int x) {
-    int lo = 0, hi = n - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (v[mid] > x) hi = mid; else lo = mid + 1;
-    }
-    return lo;
-}
-
 __global__ void __launch_bounds__(PS_THREADS, 1) paged_step_kernel(const StepParams p, const int ctas) {
     __shared__ StepShared s;
     __shared__ long long total[2];                                      // sums up to the end of the chunk

@@ -74,16 +74,6 @@ __device__ __forceinline__ bool wait_here(uint32_t bar, uint32_t parity) {
     return __all_sync(0xffffffffu, ok);
 }
 
-// smallest i with v[i] > x (v not decreasing, v[n - 1] > x)
-__device__ __forceinline__ int first_end_above(const int* v, int n, int x) {
-    int lo = 0, hi = n - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (v[mid] > x) hi = mid; else lo = mid + 1;
-    }
-    return lo;
-}
-
 struct RunFinder {
     unsigned long long rows;
     int tokens[PF_THREADS], kv[PF_THREADS], blocks_end[PF_THREADS], units[PF_THREADS], sums[2][PF_THREADS / 32];
@@ -130,7 +120,7 @@ __device__ __forceinline__ int count_chunk(const AttnParams& p, int block, int r
     const int all = load_chunk(p, block, r0, f);
     if (all < 0) return -1;
     for (int i0 = tid & ~31; i0 < all; i0 += PF_THREADS) {                   // whole numbers: the order of the additions does not matter
-        const int i = min(i0 + (tid & 31), all - 1), r = first_end_above(f.blocks_end, n, i), rb = i - (r ? f.blocks_end[r - 1] : 0);
+        const int i = min(i0 + (tid & 31), all - 1), r = first_above(f.blocks_end, n, i), rb = i - (r ? f.blocks_end[r - 1] : 0);
         const int u = i0 + (tid & 31) < all ? PrefillRuns::units(key_span(p, f.tokens[r], f.kv[r], block, rb, PF_TILE)) * p.hkv : 0;
         const int r_first = __shfl_sync(0xffffffffu, r, 0);
         if (__all_sync(0xffffffffu, r == r_first)) {                         // one request's blocks, as usual: one addition for the warp
@@ -161,7 +151,7 @@ __device__ __forceinline__ void find_run_wide(const AttnParams& p, int block, Ru
         const int all = load_chunk(p, block, 0, f);
         if (all < 0) return;
         if (all <= PF_THREADS) {                                             // a row block a thread: one more scan gives the sums and the place
-            const int r = tid < all ? first_end_above(f.blocks_end, p.batch, tid) : 0, rb = tid - (r ? f.blocks_end[r - 1] : 0);
+            const int r = tid < all ? first_above(f.blocks_end, p.batch, tid) : 0, rb = tid - (r ? f.blocks_end[r - 1] : 0);
             const int one = tid < all ? PrefillRuns::units(key_span(p, f.tokens[r], f.kv[r], block, rb, PF_TILE)) : 0, n = one * p.hkv;
             int total;
             const int e = scan_block(n, f.sums[1], total), ctas = min((int)gridDim.x, total);
