@@ -257,6 +257,7 @@ int kyb_gemv_t16_static(int fmt, const void* t16, int64_t n, int64_t k, const vo
  * kyb_paged_step: slots of a step from request lengths. Request r holds lens[r] tokens and brings new_lens[r] (negative values count as 0); pages it lacks come from
  * the top of free_pages[0, *free_count) (an array of free_cap ids), in request order, and are entered in its row of table. A request is served when its pages fit
  * the columns, its tokens the `rows` rows of the step, and the needs of the requests up to its own the free list (one that needs no page is not held up).
+ * Needs and rows count in order, served or not: one that does not fit holds up those behind it that need a page; behind more tokens than rows all are refused.
  * Out: cu_q [batch + 1] first row of each request (clipped to rows), kv_lens [batch] tokens to attend over (0: not served), positions [rows] and slots [rows] (-1:
  * not served, or a row behind the last request), lens_out [batch] (may be lens), free_count_out [1] (may be free_count), refused [1] number not served. The entries of
  * free_pages and of the table's other columns stay as they are: the same call again gives the same result unless lens_out / free_count_out are the inputs. */

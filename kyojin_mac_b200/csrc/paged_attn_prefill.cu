@@ -11,7 +11,7 @@
 // core, which runs them in that order. An item's last O has a barrier of its own: on the scores' one the next item's first scores, which wait for nothing of the softmax, could end
 // a second phase before a late softmax warp has seen the first, and a wait by parity would not pass any more. A row's reference maximum moves only when a score passes it by
 // 2^8 (bf16: 2^15), so O is rescaled (by the softmax warps themselves, in tensor memory) hardly ever; sums are of the unrounded weights, in 32 bits.
-// Measured, 64 / 8 heads of 128: 1024 tokens on 8192 cached ones 245 to 250 us, a prompt of 8192 tokens 910 us = 1210 TFLOP/s; 3200 clocks a pair of tiles, of which the tensor
+// Measured, 64 / 8 heads of 128: 1024 tokens on 8192 cached ones 241 to 250 us, a prompt of 8192 tokens 910 us = 1210 TFLOP/s; 3200 clocks a pair of tiles, of which the tensor
 // cores and the special-function units are busy 2050 each.
 // Keys that a row does not see are masked by selection in the tiles at the borders; values in places that no row of the block sees are cleared in shared memory, since such
 // places may hold anything and 0 times NaN is NaN.

@@ -630,7 +630,9 @@ def paged_step(table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor, 
     """Slots of a step from request lengths, in one launch without a word to the host. Request r holds lens[r] tokens and brings new_lens[r] (packed in request order
     into the step's `rows` rows); the pages it lacks come from the top of free_pages[:free_count] and are entered in its row of `table` [batch, columns].
     A request is served when its pages fit the columns, its tokens the rows, and the needs of the requests up to its own the free list (one that needs no page
-    is not held up); `refused` counts the others, whose lengths stay. in_place: lens and free_count are updated too (a captured step that is replayed)."""
+    is not held up); `refused` counts the others, whose lengths stay. Needs and rows count in order, served or not: a request that does not fit holds up those behind it that need a
+    page, and behind more tokens than rows all are refused, those without tokens too; leave out of a step what cannot be served (new_lens 0).
+    in_place: lens and free_count are updated too (a captured step that is replayed)."""
     dev = table.get_device()
     key = (dev, table.shape, table.is_contiguous() or table.stride(), table.dtype, lens.shape, lens.dtype, lens.is_contiguous(), new_lens.shape, new_lens.dtype, new_lens.is_contiguous(),
            free_pages.shape, free_pages.dtype, free_pages.is_contiguous(), free_count.shape, free_count.dtype, page, rows, in_place, lens.get_device(), new_lens.get_device(), free_pages.get_device(),
@@ -833,7 +835,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     kv_lens[r] - 1), keys and values through the block table [batch, columns]. Causal; window > 0: the last `window` tokens only, and the first `sinks` ones.
     cu_q does not fall: where it does so far that the requests would own more than T rows, nothing is written and `check_device_status` raises.
     max_q: the largest number of new tokens of a request (chooses the kernel; requests with more are served all the same). scale: d ** -0.5 unless given.
-    A row that sees nothing (kv_lens 0) gives zeros; rows behind the last request are left as they were (undefined without `out`). `out` is q itself
+    Keys and values that some row of a request sees are finite; other places of the cache may hold anything. A row that sees nothing (kv_lens 0) gives zeros; rows behind the last request are left as they were (undefined without `out`). `out` is q itself
     or memory apart from q and the cache. Returns out [T, heads, d]."""
     dev = q.get_device()
     key = (dev, q.shape, q.is_contiguous() or q.stride(), q.dtype, k_cache.shape, k_cache.is_contiguous() or k_cache.stride(), k_cache.dtype, v_cache.shape,
