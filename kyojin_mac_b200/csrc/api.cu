@@ -1,4 +1,4 @@
-// Status plumbing of the kyb C ABI: thread-local error text, status strings, the per-device status word.
+// Status plumbing of the kyb C ABI: thread-local error text, status strings, the per-device status word; what the launchers ask of a device.
 #include <stdarg.h>
 #include <string.h>
 
